@@ -708,6 +708,96 @@ int nnue_batch_build_halfka(const nnue_packed_position* positions, int64_t B,
                             float* outcome, float* score, int64_t* piece_count,
                             int64_t* bucket_idx, void* stream);
 
+/* ---- Bucketed ("grouped by expert") linear layers -------------------------
+ * The reference multiplies every position with the weights of all buckets and
+ * keeps the slice of its own (model/modules/stacked_linear.py:38-66); these
+ * entry points multiply each row with its own bucket's weights only, for any
+ * layer size, on 16-bit operands (with gradients) or 8-bit ones.
+ *
+ * Element types of the untyped pointers below. */
+enum { NNUE_T_F32 = 0, NNUE_T_BF16 = 1, NNUE_T_F16 = 2, NNUE_T_E4M3 = 3, NNUE_T_E5M2 = 4 };
+
+#define NNUE_GROUP_MAX_ROWS (1 << 30)
+
+/* Plan of a batch: T rows grouped by bucket.  bucket[T] (int64 with wide_ids,
+ * else int32) holds 0..E-1, or -1 for a padding row that belongs to no bucket;
+ * other ids are recorded in the device status word and treated as -1.
+ * E <= 1024.  `plan` (16-byte aligned) receives, as int32 words:
+ *   [0]                    tiles
+ *   [4 .. 4+E+1]           offsets: first place of each bucket in `order`, of
+ *                          the rows without one, and T
+ *   [4 + pad4(E+2) .. +T)  order: the rows by bucket, ascending inside a
+ *                          bucket, the rows without one last
+ * (pad4: up to the next multiple of 4) and what the products read beside
+ * them.  It depends on nothing but its inputs: the sort is stable. */
+size_t nnue_group_plan_bytes(int64_t T, int32_t E);
+int nnue_group_plan(const void* bucket, int32_t wide_ids, int64_t T, int32_t E,
+                    int32_t* plan, size_t plan_bytes, void* stream);
+
+/* dst[r, c] = src[r, c] for r < rows, c < cols; columns [cols, ldd) become zero.
+ * Between F32, BF16 and F16 (one rounding), or bytes of one 8-bit type.  The
+ * products below want rows that start at multiples of 16 bytes; this is how
+ * other rows, and fp32 parameters, get there.  Pitches in elements. */
+int nnue_pack_rows(const void* src, int32_t src_type, int64_t lds, void* dst,
+                   int32_t dst_type, int64_t ldd, int64_t rows, int64_t cols,
+                   void* stream);
+
+/* y[p, n]  = sum_k x[p, k] w[b, n, k] + bias[b, n],  b = bucket of row p
+ * dx[p, k] = sum_n dy[p, n] w[b, n, k]
+ * dw[b, n, k] = sum_{p of b} dy[p, n] x[p, k],  dbias[b, n] = sum_{p of b} dy[p, n]
+ * x [T, K], w [E, N, K], dy [T, N] of `type` (BF16 or F16), rows at pitches ldx,
+ * ldw, lddy (elements) that are multiples of 16 bytes; bias [E, N] of any of the
+ * three float types, may be NULL; y [T, N], dx [T, K] and dw [E, N, K] contiguous,
+ * y and dw of `type` or F32, dx of `type`, dbias [E, N] of any float type, may be
+ * NULL.  Sums are fp32, rounded once.  Rows without a bucket get zeros in y and
+ * dx, whatever they hold; a bucket without rows gets zeros in dw and dbias.  Sums
+ * run in an order that the sizes alone fix: results are reproducible.  T = 0 is
+ * allowed.  `plan`: nnue_group_plan's, of the same T and E. */
+int nnue_grouped_linear_fwd(const void* x, int64_t ldx, const void* w,
+                            int64_t ldw, const void* bias, int32_t bias_type,
+                            const void* plan, void* y, int32_t y_type, int64_t T,
+                            int64_t K, int64_t N, int32_t E, int32_t type,
+                            void* stream);
+int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, const void* w,
+                                  int64_t ldw, const void* plan, void* dx,
+                                  int64_t T, int64_t K, int64_t N, int32_t E,
+                                  int32_t type, void* stream);
+int nnue_grouped_linear_bwd_weight(const void* dy, int64_t lddy, const void* x,
+                                   int64_t ldx, const void* plan, void* dw,
+                                   int32_t dw_type, void* dbias,
+                                   int32_t dbias_type, int64_t T, int64_t K,
+                                   int64_t N, int32_t E, int32_t type,
+                                   void* stream);
+
+/* 8-bit floating point with a scale per block of 128.  For each block
+ * (a = its largest finite |v|, MAX = 448 for E4M3, 57344 for E5M2):
+ *   scale = 2^ceil(log2(a / MAX)), 1 for a = 0, at least 2^-126
+ *   q = v / scale to the nearest number of the format, ties to even
+ * Numbers that are not finite become NaN in E4M3 and stay what they are in E5M2.
+ * rows:  x [T, K] (F32, BF16 or F16, pitch ldx) -> q [T, K] (pitch ldq, at most
+ *        the row length rounded up to 128; columns [K, ldq) become zero),
+ *        scale [T, ceil(K / 128)]
+ * tiles: w [E, N, K] (pitch ldw) -> q [E, N, K], scale [E, ceil(N / 128),
+ *        ceil(K / 128)]; tiles start anew in every bucket. */
+int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, void* q,
+                           int64_t ldq, float* scale, int64_t T, int64_t K,
+                           int32_t format, void* stream);
+int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
+                            int64_t ldq, float* scale, int32_t E, int64_t N,
+                            int64_t K, int32_t format, void* stream);
+
+/* y[p, n] = sum_c x_scale[p, c] w_scale[b, n / 128, c]
+ *                 sum_{k in block c} x[p, k] w[b, n, k]  + bias[b, n]
+ * x [T, K] and w [E, N, K] of one 8-bit format, pitches that are multiples of 16,
+ * scales as the quantisers lay them out (any fp32 values, not only powers of
+ * two), bias [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are
+ * fp32.  plan NULL: E = 1 and every row belongs to the one matrix. */
+int nnue_fp8_linear_fwd(const void* x, int64_t ldx, const float* x_scale,
+                        const void* w, int64_t ldw, const float* w_scale,
+                        const float* bias, const void* plan, void* y,
+                        int32_t y_type, int64_t T, int64_t K, int64_t N,
+                        int32_t E, int32_t format, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,10 @@ SOURCES = [
     "layer_stack_weights.cu",
     "batch_build.cu",
     "sf_loss.cu",
+    "group_plan.cu",
+    "grouped_linear.cu",
+    "fp8_blocks.cu",
+    "fp8_linear.cu",
 ]
 
 NVCC_FLAGS = [

@@ -1,0 +1,274 @@
+// Plan of a batch for the bucketed matrix products: rows grouped by bucket (a stable counting sort), the first place of
+// every bucket, and the list of tiles of at most 128 rows of one bucket that the products walk.
+//
+// Mathematics: place(p) = #{q : b(q) < b(p)} + #{q < p : b(q) = b(p)}.  A warp takes 32 consecutive rows at a time, so
+// the second term is a histogram of the rows before its slice plus the lanes below it that hold the same bucket
+// (one match instruction).  Work: ids read twice, order written once; bound by latency up to about a million rows.
+//
+// Batches of at most kSingleRows rows take ONE launch of one block (1024 threads, a counter per warp and bucket in shared
+// memory).  Longer ones take three: counters per block of rows, their scan, the fill; the launches cost about 2.5 us each,
+// which one block needs for some ten thousand rows.
+#include "grouped.cuh"
+
+namespace nnue {
+
+constexpr int kGpThreads = 1024;
+constexpr int kGpWarps = kGpThreads / 32;
+constexpr int64_t kSingleRows = 16384;
+constexpr int kBlockRows = 4096;  // rows per block of the long form
+
+// bin of a row: its bucket, or E for -1 (padding row) and, with a note in the status word, for an id out of range
+template <typename Id>
+__device__ __forceinline__ int group_bin(const Id* bucket, int64_t p, int E, unsigned long long* status) {
+    const Id b = bucket[p];
+    if (b >= 0 && b < (Id)E) return (int)b;
+    if (b != (Id)-1 && status) note_bad_index(status);
+    return E;
+}
+
+// counters of each warp's slice of rows [lo, hi): hist[warp][bin]
+template <typename Id>
+__device__ __forceinline__ void group_histogram(const Id* bucket, int64_t lo, int64_t hi, int bins, int32_t* hist,
+                                                unsigned long long* status) {
+    for (int i = threadIdx.x; i < bins * kGpWarps; i += kGpThreads) hist[i] = 0;
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t per = (hi - lo + kGpWarps * 32 - 1) / (kGpWarps * 32) * 32;
+    const int64_t a = lo + warp * per, b = min(hi, a + per);
+    for (int64_t p = a + lane; p < b; p += 32) atomicAdd(hist + warp * bins + group_bin(bucket, p, bins - 1, status), 1);
+    __syncthreads();
+}
+
+// hist[w][bin] becomes the number of rows of `bin` in the slices before w; returns the bin's total
+__device__ __forceinline__ int group_scan_warps(int32_t* hist, int bins, int bin) {
+    int run = 0;
+#pragma unroll 8
+    for (int w = 0; w < kGpWarps; ++w) {
+        const int v = hist[w * bins + bin];
+        hist[w * bins + bin] = run;
+        run += v;
+    }
+    return run;
+}
+
+// rows of this block to their places: base[bin] + hist[warp][bin] + rank among the warp's 32
+template <typename Id>
+__device__ __forceinline__ void group_fill(const Id* bucket, int64_t lo, int64_t hi, int bins, int32_t* hist,
+                                           const int32_t* base, int32_t* order) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t per = (hi - lo + kGpWarps * 32 - 1) / (kGpWarps * 32) * 32;
+    const int64_t a = lo + warp * per, b = min(hi, a + per);
+    int32_t* mine = hist + warp * bins;
+    for (int64_t p0 = a; p0 < b; p0 += 32) {
+        const int64_t p = p0 + lane;
+        const bool live = p < b;
+        const int bin = live ? group_bin(bucket, p, bins - 1, nullptr) : -1;
+        const unsigned same = __match_any_sync(kFullMask, bin);
+        const int rank = __popc(same & ((1u << lane) - 1u));
+        int at = 0;
+        if (live) at = mine[bin];
+        __syncwarp();
+        if (live) {
+            order[base[bin] + at + rank] = (int32_t)p;
+            if (rank == 0) mine[bin] = at + __popc(same);
+        }
+        __syncwarp();
+    }
+}
+
+// exclusive scan over the block of one pair of values per thread; the totals go to `total`
+__device__ __forceinline__ int2 block_scan2(int2 v, int2* s_warp, int2* total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int2 inc = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(kFullMask, inc.x, d), y = __shfl_up_sync(kFullMask, inc.y, d);
+        if (lane >= d) { inc.x += x; inc.y += y; }
+    }
+    __syncthreads();
+    if (lane == 31) s_warp[warp] = inc;
+    __syncthreads();
+    if (warp == 0) {
+        int2 w = s_warp[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(kFullMask, w.x, d), y = __shfl_up_sync(kFullMask, w.y, d);
+            if (lane >= d) { w.x += x; w.y += y; }
+        }
+        s_warp[lane] = w;
+    }
+    __syncthreads();
+    const int2 before = warp ? s_warp[warp - 1] : make_int2(0, 0);
+    *total = s_warp[kGpWarps - 1];
+    return make_int2(before.x + inc.x - v.x, before.y + inc.y - v.y);
+}
+
+// Totals of the bins (s_total) to the plan's offsets and tile list; s_base[bin] = first place, s_tile[bin] = first tile.
+__device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_total, int32_t* s_base, int32_t* s_tile,
+                                            int2* s_warp, int32_t* plan) {
+    const int bins = E + 1;
+    int2 carry = make_int2(0, 0);
+    for (int b0 = 0; b0 < bins; b0 += kGpThreads) {
+        const int b = b0 + threadIdx.x;
+        const int n = b < bins ? s_total[b] : 0;
+        int2 total;
+        const int2 ex = block_scan2(make_int2(n, (n + kGroupRows - 1) / kGroupRows), s_warp, &total);
+        if (b < bins) {
+            s_base[b] = carry.x + ex.x;
+            s_tile[b] = carry.y + ex.y;
+            plan[group_offsets_at() + b] = carry.x + ex.x;
+        }
+        carry.x += total.x;
+        carry.y += total.y;
+    }
+    if (threadIdx.x == 0) {
+        s_tile[bins] = carry.y;
+        plan[0] = carry.y;
+        plan[group_offsets_at() + bins] = (int32_t)T;
+    }
+    __syncthreads();
+    int4* tiles = reinterpret_cast<int4*>(plan + group_tiles_at(T, E));
+    for (int t = threadIdx.x; t < s_tile[bins]; t += kGpThreads) {
+        int lo = 0, hi = bins - 1;  // the last bin whose first tile is not behind t; empty bins share a first tile
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_tile[mid] <= t) lo = mid;
+            else hi = mid - 1;
+        }
+        const int at = (t - s_tile[lo]) * kGroupRows;
+        tiles[t] = make_int4(lo, s_base[lo] + at, min(kGroupRows, s_total[lo] - at), 0);
+    }
+}
+
+constexpr size_t group_smem_bytes(int bins) { return sizeof(int32_t) * ((size_t)bins * kGpWarps + 3 * (size_t)bins + 2); }
+
+template <typename Id>
+__global__ void __launch_bounds__(kGpThreads)
+    k_group_single(const Id* __restrict__ bucket, int64_t T, int E, int32_t* __restrict__ plan, unsigned long long* status) {
+    extern __shared__ int32_t s_hist[];
+    const int bins = E + 1;
+    int32_t* s_total = s_hist + bins * kGpWarps;
+    int32_t* s_base = s_total + bins;
+    int32_t* s_tile = s_base + bins;  // [bins + 1]
+    __shared__ int2 s_warp[kGpWarps];
+    group_histogram(bucket, 0, T, bins, s_hist, status);
+    for (int b = threadIdx.x; b < bins; b += kGpThreads) s_total[b] = group_scan_warps(s_hist, bins, b);
+    __syncthreads();
+    group_tiles(T, E, s_total, s_base, s_tile, s_warp, plan);
+    group_fill(bucket, 0, T, bins, s_hist, s_base, plan + group_order_at(E));
+}
+
+// long form, 1: counts[bin][block]
+template <typename Id>
+__global__ void __launch_bounds__(kGpThreads)
+    k_group_count(const Id* __restrict__ bucket, int64_t T, int E, int32_t* __restrict__ counts, unsigned long long* status) {
+    extern __shared__ int32_t s_hist[];
+    const int bins = E + 1;
+    const int64_t lo = (int64_t)blockIdx.x * kBlockRows, hi = min(T, lo + kBlockRows);
+    group_histogram(bucket, lo, hi, bins, s_hist, status);
+    for (int b = threadIdx.x; b < bins; b += kGpThreads)
+        counts[(int64_t)b * gridDim.x + blockIdx.x] = group_scan_warps(s_hist, bins, b);
+}
+
+// long form, 2: counts[bin][block] becomes the number of rows of `bin` in the blocks before, and the plan's head
+__global__ void __launch_bounds__(kGpThreads)
+    k_group_scan(int64_t T, int E, int blocks, int32_t* __restrict__ counts, int32_t* __restrict__ plan) {
+    extern __shared__ int32_t s_total[];
+    const int bins = E + 1;
+    int32_t* s_base = s_total + bins;
+    int32_t* s_tile = s_base + bins;
+    __shared__ int2 s_warp[kGpWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int b = warp; b < bins; b += kGpWarps) {
+        int run = 0;
+        for (int i0 = 0; i0 < blocks; i0 += 32) {
+            const int i = i0 + lane;
+            const int v = i < blocks ? counts[(int64_t)b * blocks + i] : 0;
+            int inc = v;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(kFullMask, inc, d);
+                if (lane >= d) inc += x;
+            }
+            if (i < blocks) counts[(int64_t)b * blocks + i] = run + inc - v;
+            run += __shfl_sync(kFullMask, inc, 31);
+        }
+        if (lane == 0) s_total[b] = run;
+    }
+    __syncthreads();
+    group_tiles(T, E, s_total, s_base, s_tile, s_warp, plan);
+}
+
+// long form, 3: rows to their places
+template <typename Id>
+__global__ void __launch_bounds__(kGpThreads)
+    k_group_fill(const Id* __restrict__ bucket, int64_t T, int E, const int32_t* __restrict__ counts, int32_t* __restrict__ plan) {
+    extern __shared__ int32_t s_hist[];
+    const int bins = E + 1;
+    int32_t* s_base = s_hist + bins * kGpWarps;
+    const int64_t lo = (int64_t)blockIdx.x * kBlockRows, hi = min(T, lo + kBlockRows);
+    group_histogram(bucket, lo, hi, bins, s_hist, nullptr);
+    for (int b = threadIdx.x; b < bins; b += kGpThreads) {
+        group_scan_warps(s_hist, bins, b);
+        s_base[b] = plan[group_offsets_at() + b] + counts[(int64_t)b * gridDim.x + blockIdx.x];
+    }
+    __syncthreads();
+    group_fill(bucket, lo, hi, bins, s_hist, s_base, plan + group_order_at(E));
+}
+
+inline int64_t group_blocks(int64_t T) { return T <= kSingleRows ? 0 : (T + kBlockRows - 1) / kBlockRows; }
+
+template <typename Id>
+int launch_plan(const Id* bucket, int64_t T, int32_t E, int32_t* plan, unsigned long long* status, cudaStream_t s) {
+    const int bins = E + 1;
+    const size_t smem = group_smem_bytes(bins);
+    static bool opted[64] = {};  // more than 48 KB of dynamic shared memory needs the opt-in, once per device
+    int dev = 0;
+    NNUE_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !opted[dev]) {
+        const int most = (int)group_smem_bytes(kMaxGroups + 1);
+        NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_single<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_count<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_fill<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        if (dev >= 0 && dev < 64) opted[dev] = true;
+    }
+    const int64_t blocks = group_blocks(T);
+    if (blocks == 0) {
+        k_group_single<Id><<<1, kGpThreads, smem, s>>>(bucket, T, E, plan, status);
+        note_launches(1);
+    } else {
+        int32_t* counts = plan + group_counts_at(T, E);
+        k_group_count<Id><<<(unsigned)blocks, kGpThreads, smem, s>>>(bucket, T, E, counts, status);
+        k_group_scan<<<1, kGpThreads, sizeof(int32_t) * (3 * bins + 2), s>>>(T, E, (int)blocks, counts, plan);
+        k_group_fill<Id><<<(unsigned)blocks, kGpThreads, smem, s>>>(bucket, T, E, counts, plan);
+        note_launches(3);
+    }
+    NNUE_CUDA_TRY(cudaGetLastError());
+    return NNUE_OK;
+}
+
+}  // namespace nnue
+
+using namespace nnue;
+
+extern "C" size_t nnue_group_plan_bytes(int64_t T, int32_t E) {
+    if (T < 0 || T > NNUE_GROUP_MAX_ROWS || E <= 0 || E > kMaxGroups) return 0;
+    return sizeof(int32_t) * (size_t)(group_counts_at(T, E) + group_blocks(T) * (E + 1));
+}
+
+extern "C" int nnue_group_plan(const void* bucket, int32_t wide_ids, int64_t T, int32_t E, int32_t* plan, size_t plan_bytes,
+                               void* stream) {
+    NNUE_REQUIRE(T >= 0 && E > 0, NNUE_ERR_ARG, "nnue_group_plan: negative batch or no bucket");
+    NNUE_REQUIRE(E <= kMaxGroups && T <= NNUE_GROUP_MAX_ROWS, NNUE_ERR_UNSUPPORTED,
+                 "nnue_group_plan: %d buckets (at most %d) of %lld rows (at most %lld)", E, kMaxGroups, (long long)T,
+                 (long long)NNUE_GROUP_MAX_ROWS);
+    NNUE_REQUIRE(T == 0 || bucket, NNUE_ERR_ARG, "nnue_group_plan: null bucket list");
+    NNUE_REQUIRE(plan && plan_bytes >= nnue_group_plan_bytes(T, E) && aligned16(plan), NNUE_ERR_WORKSPACE,
+                 "nnue_group_plan: plan buffer too small or unaligned");
+    unsigned long long* status = device_status_ptr();
+    NNUE_REQUIRE(status, NNUE_ERR_CUDA, "nnue_group_plan: no device status word");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    ProfScope prof("group_plan", s);
+    return wide_ids ? launch_plan(static_cast<const int64_t*>(bucket), T, E, plan, status, s)
+                    : launch_plan(static_cast<const int32_t*>(bucket), T, E, plan, status, s);
+}

@@ -1,0 +1,73 @@
+// Shared declarations of the bucketed ("grouped by expert") matrix products: the plan of a batch, the element types of
+// the C ABI and conversions between them.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace nnue {
+
+constexpr int kGroupRows = 128;       // rows per tile of the plan: M of the tensor-core instructions
+constexpr int kMaxGroups = 1024;
+
+__host__ __device__ inline int64_t pad4(int64_t n) { return (n + 3) / 4 * 4; }
+
+// A tile of the plan: `count` rows (1..128) of one bucket, at order[start].  bucket == groups: rows of no bucket.
+struct GroupTile {
+    int32_t bucket, start, count, pad;
+};
+
+struct GroupPlanView {
+    const int32_t* n_tiles;   // [1]
+    const int32_t* offsets;   // [E + 2]: first place of each bucket in `order`, of the rows without one, T
+    const int32_t* order;     // [T] rows by bucket, in their own order inside a bucket
+    const GroupTile* tiles;   // [<= group_max_tiles]
+};
+
+__host__ __device__ inline int64_t group_max_tiles(int64_t T, int32_t E) {
+    const int64_t by_rows = (T + kGroupRows - 1) / kGroupRows + E + 1;
+    return by_rows < T ? by_rows : T;  // every tile holds a row
+}
+
+// int32 words: [0] tiles, [4..] offsets, order, tiles, then the counters of the launches for long batches
+__host__ __device__ inline int64_t group_offsets_at() { return 4; }
+__host__ __device__ inline int64_t group_order_at(int32_t E) { return 4 + pad4(E + 2); }
+__host__ __device__ inline int64_t group_tiles_at(int64_t T, int32_t E) { return group_order_at(E) + pad4(T); }
+__host__ __device__ inline int64_t group_counts_at(int64_t T, int32_t E) {
+    return group_tiles_at(T, E) + 4 * group_max_tiles(T, E);
+}
+
+__host__ __device__ inline GroupPlanView group_view(const void* plan, int64_t T, int32_t E) {
+    const int32_t* p = static_cast<const int32_t*>(plan);
+    GroupPlanView v;
+    v.n_tiles = p;
+    v.offsets = p + group_offsets_at();
+    v.order = p + group_order_at(E);
+    v.tiles = reinterpret_cast<const GroupTile*>(p + group_tiles_at(T, E));
+    return v;
+}
+
+inline int type_bytes(int32_t t) { return t == NNUE_T_F32 ? 4 : (t == NNUE_T_BF16 || t == NNUE_T_F16) ? 2 : 1; }
+inline bool is_float_type(int32_t t) { return t == NNUE_T_F32 || t == NNUE_T_BF16 || t == NNUE_T_F16; }
+inline bool is_half_type(int32_t t) { return t == NNUE_T_BF16 || t == NNUE_T_F16; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ bool type_is_byte(int32_t t) { return t == NNUE_T_E4M3 || t == NNUE_T_E5M2; }
+
+// element `i` of an array of type `t` (F32, BF16 or F16) as fp32; exact
+__device__ __forceinline__ float load_as_float(const void* p, int32_t t, int64_t i) {
+    if (t == NNUE_T_F32) return __ldg(static_cast<const float*>(p) + i);
+    if (t == NNUE_T_BF16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
+    return __half2float(__ldg(static_cast<const __half*>(p) + i));
+}
+// one rounding (to nearest, ties to even), none for F32
+__device__ __forceinline__ void store_from_float(void* p, int32_t t, int64_t i, float v) {
+    if (t == NNUE_T_F32) static_cast<float*>(p)[i] = v;
+    else if (t == NNUE_T_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+#endif
+
+}  // namespace nnue

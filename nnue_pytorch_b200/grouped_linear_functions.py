@@ -1,0 +1,175 @@
+"""Bucketed ("grouped by expert") linear layers on 16-bit operands.
+
+`GroupPlan` groups the rows of a batch by their bucket; `grouped_linear` multiplies every row with the weights of its own
+bucket and has gradients for the rows, the weights and the bias.  Any number of buckets up to 1024, any layer size; the
+reference multiplies every row with all buckets' weights and selects afterwards (model/modules/stacked_linear.py:38-66).
+
+    plan = GroupPlan(bucket, count)                      # int64 or int32 [T]; -1: a padding row of no bucket
+    y = grouped_linear(x, weight, bias, plan)            # x [T, K], weight [count * N, K], bias [count * N]
+
+Operands are bf16 or fp16, sums fp32.  fp32 parameters (weight, bias) are allowed: the weights are rounded to the
+rows' type for the products, their gradients come back in fp32, unrounded.  One plan serves every layer and direction
+of its batch.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import autograd
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._launch import _NO_SPAN, _ptr, _require_cuda, _span, _stream
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.float8_e5m2: 4}
+HALF = (torch.bfloat16, torch.float16)
+
+
+def _on(dev: torch.device):
+    """Context in which `dev` is the current device (nothing to do when it already is)."""
+    return _NO_SPAN if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _pad4(n: int) -> int:
+    return (n + 3) // 4 * 4
+
+
+class GroupPlan:
+    """Rows of a batch grouped by bucket (`nnue_group_plan`): a stable sort.
+
+    order    int32 [T]: the rows by bucket, ascending inside a bucket, rows of no bucket (-1) last
+    offsets  int32 [count + 1]: first place of every bucket in `order`, and the number of rows that have one
+
+    An id below -1 or from `count` on is treated as -1 and recorded in the device status word
+    (`_lib.device_status`).  The plan is built on the current stream and holds no reference to `bucket`."""
+
+    __slots__ = ("rows", "count", "device", "buffer")
+
+    @torch.compiler.disable
+    def __init__(self, bucket: torch.Tensor, count: int):
+        dev = _require_cuda(bucket)
+        assert bucket.dtype in (torch.int64, torch.int32), "bucket ids are int64 or int32"
+        count = int(count)
+        assert 1 <= count <= 1024, "1 to 1024 buckets"
+        bucket = bucket.detach().reshape(-1).contiguous()
+        lib = _lib.load()
+        self.rows, self.count, self.device = bucket.numel(), count, dev
+        nbytes = lib.nnue_group_plan_bytes(self.rows, count)
+        self.buffer = torch.empty(max(nbytes // 4, 4), dtype=torch.int32, device=dev)
+        with _on(dev), _span("group_plan", dev):
+            st = lib.nnue_group_plan(_ptr(bucket), bucket.dtype == torch.int64, self.rows, count, _ptr(self.buffer), nbytes,
+                                     _stream(dev))
+        _lib.check(st, "nnue_group_plan")
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self.buffer[4 : 5 + self.count]
+
+    @property
+    def order(self) -> torch.Tensor:
+        at = 4 + _pad4(self.count + 2)
+        return self.buffer[at : at + self.rows]
+
+    def check(self, t: torch.Tensor) -> None:
+        assert t.shape[0] == self.rows, f"the plan was built for {self.rows} rows, not {t.shape[0]}"
+        assert t.device == self.device, "the plan lives on another device"
+
+
+def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev) -> tuple[torch.Tensor, int]:
+    """(t as rows of `dtype` that start at multiples of 16 bytes, their pitch in elements): `t` itself where it is one,
+    else a copy whose rows are padded with zeros (`nnue_pack_rows`)."""
+    rows, cols = t.shape
+    unit = 16 // dtype.itemsize
+    if t.dtype == dtype and (cols == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0:
+        pitch = t.stride(0)
+        if pitch % unit == 0 and pitch >= cols:
+            return t, pitch
+        if rows == 1 and cols % unit == 0:
+            return t, cols
+    if cols > 1 and t.stride(1) != 1 or t.stride(0) < cols:
+        t = t.contiguous()
+    pitch = (cols + unit - 1) // unit * unit
+    out = torch.empty(rows, pitch, dtype=dtype, device=dev)
+    if t.dtype.itemsize != 1:
+        st = lib.nnue_pack_rows(_ptr(t), TYPES[t.dtype], t.stride(0), _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
+    else:
+        assert t.dtype == dtype
+        st = lib.nnue_pack_rows(_ptr(t), TYPES[dtype], t.stride(0), _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
+    _lib.check(st, "nnue_pack_rows")
+    return out, pitch
+
+
+class GroupedLinearFunction(autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, plan, out_dtype=None):
+        dev = _require_cuda(x, weight) if bias is None else _require_cuda(x, weight, bias)
+        dtype = x.dtype
+        assert dtype in HALF, "rows are bf16 or fp16"
+        assert weight.dtype in (dtype, torch.float32), "weights have the rows' type or are fp32"
+        out_dtype = out_dtype or dtype
+        assert out_dtype in (dtype, torch.float32), "the output has the rows' type or is fp32"
+        assert x.dim() == 2 and weight.dim() in (2, 3)
+        plan.check(x)
+        E = plan.count
+        w2 = weight.detach().flatten(0, 1) if weight.dim() == 3 else weight.detach()
+        T, K = x.shape
+        N = w2.shape[0] // E
+        assert K >= 1 and N >= 1 and w2.shape == (E * N, K) and (weight.dim() == 2 or weight.shape[0] == E), \
+            f"weight {tuple(weight.shape)} does not hold {E} layers of {K} inputs"
+        if bias is not None:
+            assert bias.dtype in (dtype, torch.float32) and bias.numel() == E * N
+        lib = _lib.load()
+        y = torch.empty(T, N, dtype=out_dtype, device=dev)
+        with _on(dev), _span("grouped_linear_fwd", dev):
+            xr, ldx = _pitched(x.detach(), dtype, lib, dev)
+            wr, ldw = _pitched(w2, dtype, lib, dev)
+            b = None if bias is None else bias.detach().contiguous()
+            st = lib.nnue_grouped_linear_fwd(
+                _ptr(xr), ldx, _ptr(wr), ldw, _ptr(b), 0 if b is None else TYPES[b.dtype], _ptr(plan.buffer), _ptr(y),
+                TYPES[out_dtype], T, K, N, E, TYPES[dtype], _stream(dev))
+        _lib.check(st, "nnue_grouped_linear_fwd")
+        ctx.save_for_backward(xr, wr, plan.buffer)
+        ctx.dims = (T, K, N, E, ldx, ldw)
+        ctx.dtype, ctx.w_like, ctx.b_like = dtype, (weight.dtype, weight.shape), None if bias is None else (bias.dtype, bias.shape)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, plan = ctx.saved_tensors
+        T, K, N, E, ldx, ldw = ctx.dims
+        dev, dtype = x.device, ctx.dtype
+        lib = _lib.load()
+        dx = dw = db = None
+        with _on(dev), _span("grouped_linear_bwd", dev):
+            s = _stream(dev)
+            dyr, lddy = _pitched(dy, dtype, lib, dev)
+            if ctx.needs_input_grad[0]:
+                dx = torch.empty(T, K, dtype=dtype, device=dev)
+                _lib.check(lib.nnue_grouped_linear_bwd_input(_ptr(dyr), lddy, _ptr(w), ldw, _ptr(plan), _ptr(dx), T, K, N, E,
+                                                             TYPES[dtype], s), "nnue_grouped_linear_bwd_input")
+            need_b = ctx.needs_input_grad[2] and ctx.b_like is not None
+            if ctx.needs_input_grad[1] or need_b:
+                w_dtype, w_shape = ctx.w_like
+                dw = torch.empty(E * N, K, dtype=w_dtype, device=dev)
+                if need_b:
+                    db = torch.empty(ctx.b_like[1], dtype=ctx.b_like[0], device=dev)
+                _lib.check(lib.nnue_grouped_linear_bwd_weight(
+                    _ptr(dyr), lddy, _ptr(x), ldx, _ptr(plan), _ptr(dw), TYPES[w_dtype], _ptr(db),
+                    0 if db is None else TYPES[db.dtype], T, K, N, E, TYPES[dtype], s), "nnue_grouped_linear_bwd_weight")
+                dw = dw.view(w_shape) if ctx.needs_input_grad[1] else None
+        return dx, dw, db, None, None
+
+
+@torch.compiler.disable  # ctypes launches: runs eagerly inside a compiled model
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, plan: GroupPlan,
+                   out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y[p] = weight[b(p)] x[p] + bias[b(p)], zeros for rows of no bucket.
+
+    x       bf16 or fp16 [T, K], any strides (rows that do not start at multiples of 16 bytes are copied first)
+    weight  [count * N, K] or [count, N, K], of x's type or fp32
+    bias    count * N numbers of x's type or fp32, or None
+    out_dtype  x's type (default) or float32
+
+    Gradients: those of the formula, with dy rounded to x's type where it is fp32; each in its tensor's own type."""
+    return GroupedLinearFunction.apply(x, weight, bias, plan, out_dtype)
