@@ -6,6 +6,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace nnue {
 
@@ -96,6 +97,35 @@ int sm_count() {
         cache[dev] = n;
     }
     return cache[dev];
+}
+
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+               const uint64_t* strides, const uint32_t* box) {
+    typedef decltype(&cuTensorMapEncodeTiled) Encode;
+    static Encode encode = nullptr;  // the library does not link against libcuda: the driver's entry point, looked up once
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        NNUE_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        NNUE_REQUIRE(found == cudaDriverEntryPointSuccess && fn, NNUE_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+        encode = reinterpret_cast<Encode>(fn);
+    }
+    const cuuint32_t ones[3] = {1, 1, 1};
+    auto call = [&] {
+        return encode(map, type, (cuuint32_t)rank, const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(dims),
+                      reinterpret_cast<const cuuint64_t*>(strides), box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // a thread that has made no runtime call yet (an autograd worker): bind the device's context to it
+        int dev = 0;
+        NNUE_CUDA_TRY(cudaGetDevice(&dev));
+        NNUE_CUDA_TRY(cudaSetDevice(dev));
+        r = call();
+    }
+    NNUE_REQUIRE(r == CUDA_SUCCESS, NNUE_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return NNUE_OK;
 }
 
 // ---- gradient norm helpers ------------------------------------------------

@@ -68,6 +68,8 @@ CASES = [
     (1, 1, 1, 1), (1, 8, 64, 32), (2, 3, 17, 5), (5, 2, 8, 1), (40, 8, 100, 1), (127, 1, 64, 31), (128, 1, 128, 128), (129, 1, 130, 129),
     (300, 3, 96, 200), (257, 64, 72, 40), (1000, 8, 1000, 32), (700, 5, 264, 520), (64, 70, 520, 33), (3, 1, 4099, 260),
     (2000, 2, 40, 300), (515, 4, 1032, 257),
+    # more tiles than SMs, in every direction
+    (9000, 8, 256, 2100), (24000, 3, 1000, 520), (5000, 40, 520, 520),
 ]
 
 
@@ -264,6 +266,31 @@ def test_other_stream_and_replayed_graph(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(want[s - 1], out))
     del graph
+
+
+def test_from_threads_of_their_own(dev):
+    """Threads that have made no CUDA call yet (as autograd's are), two at a time."""
+    import threading
+
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator().manual_seed(12)
+    b = _ids(256, 4, 12).to(dev)
+    x, w = torch.randn(256, 64, generator=g).bfloat16().to(dev), torch.randn(4 * 64, 64, generator=g).bfloat16().to(dev)
+    plan = GroupPlan(b, 4)
+    want = grouped_linear(x, w, None, plan)
+    got = [None, None]
+
+    def work(i):
+        with torch.no_grad():
+            got[i] = [grouped_linear(x, w, None, plan) for _ in range(20)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(y, want) for ys in got for y in ys)
 
 
 def test_offsets_beyond_32_bits(dev):
