@@ -4,15 +4,16 @@
 //   weight gradient  dw[b, n, k] = sum_{p of b} dy[p, n] x[p, k],  dbias[b, n] = sum_{p of b} dy[p, n]
 //
 // One kernel, three ways to read its operands; D (128 rows x BN columns) accumulates in tensor memory in fp32.
-//   forward   A = 128 rows of x of one bucket, gathered by the plan (four rows per copy), K-major;   B = rows of w, K-major
+//   forward   A = 128 rows of x of one bucket, gathered by the plan, K-major;   B = rows of w, K-major
 //   dx        A = 128 rows of dy, gathered, K-major;                       B = columns of w, MN-major (w is read as it lies)
 //   dw        A = columns of dy, B = columns of x, both MN-major; the sum runs over the bucket's rows, gathered
-// Rows behind the end of a bucket are named by an index outside the map, which the copy engine reads as zeros: nothing is
-// masked in the loop, and no row of another bucket is ever multiplied.
+// Rows behind the end of a bucket are zeros where the sum runs over rows and never read elsewhere; no row of another bucket
+// is ever multiplied.  (Gathering with TMA, four rows per copy, was measured first: about 75 cycles per copy and SM whatever
+// issues it, 675 us for the forward of 16384 x 4096 x 2048 and 1700 for its dw.)
 //
-// Roles: warp 0 copies (TMA into a ring of shared-memory stages, 128 bytes of K or of M/N per row, swizzled), one thread
-// of warp 1 issues the instructions, warps 2-5 bring finished tiles out while the next tile multiplies (two accumulators),
-// and in dw warps 6-9 add up the bias gradient from the same stages.  Persistent: a CTA per SM walks the tiles with a
+// Roles: warps 0-3 copy into a ring of shared-memory stages (128 bytes of K or of M/N per row, swizzled; gathered rows 16
+// bytes per thread, w as TMA boxes), one thread of warp 4 issues the instructions, warps 5-8 bring finished tiles out while
+// the next tile multiplies (two accumulators), and in dw warps 9-12 add up the bias gradient from the same stages.  Persistent: a CTA per SM walks the tiles with a
 // stride of the grid.  With few tiles the sum is split over a cluster of 2 to 8 CTAs, whose partial tiles meet in
 // distributed shared memory and are added in the order of their ranks.  All orders are fixed by the sizes: results are
 // reproducible.  Every wait is bounded; one that runs out raises the device status word and the CTA leaves, its tensor
@@ -31,13 +32,15 @@ constexpr int kGlStageWarp = 4096;           // staging of one output warp: 32 r
 
 constexpr int gl_stages(int bn) { return bn == 256 ? 4 : bn == 128 ? 6 : 8; }
 constexpr int gl_stage_bytes(int bn) { return kGlABytes + bn * 128; }
-constexpr int gl_threads(int mode) { return mode == kModeDw ? 320 : 192; }
+constexpr int gl_threads(int mode) { return mode == kModeDw ? 416 : 288; }
 constexpr int gl_smem(int bn) {  // alignment, ring, staging, bias per output warp, bias gradient, barriers
     return 1024 + gl_stages(bn) * gl_stage_bytes(bn) + 4 * kGlStageWarp + 4 * bn * 4 + kGroupRows * 4 + 256;
 }
 
 struct GlArgs {
     GroupPlanView plan;
+    const unsigned char *rows_a, *rows_b;  // gathered operands: x (forward), dy (dx), dy and x (dw)
+    int64_t pitch_a, pitch_b;              // bytes
     void* out;
     void* sums;              // dw: dbias, or null
     const void* bias;        // forward, or null
@@ -200,80 +203,80 @@ __device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bo
     }
 }
 
-// ---- warp 0: copies ---------------------------------------------------------------------------------------------------
+// ---- warps 0-3: copies ------------------------------------------------------------------------------------------------
+// Gathered rows come 16 bytes per thread and copy: eight neighbouring threads read 128 bytes of one row, a thread serves
+// rows j / 8 + 16 i.  Copies announce themselves on the stage's barrier when they land; the thread does not wait.
 template <int MODE, int BN, bool SPLIT>
-__device__ __forceinline__ bool gl_copy_role(const GlArgs& a, const CUtensorMap* map_a, const CUtensorMap* map_b, uint32_t ring,
-                                             uint64_t* full, uint64_t* empty, int t0, int stride, int tiles, int rank, int ranks) {
+__device__ __forceinline__ bool gl_copy_role(const GlArgs& a, const CUtensorMap* map_b, uint32_t ring, uint64_t* full,
+                                             uint64_t* empty, int t0, int stride, int tiles, int rank, int ranks) {
     constexpr int S = gl_stages(BN);
-    const int lane = threadIdx.x & 31;
+    const int j = threadIdx.x, lane = j & 31, piece = j & 7, r0 = j >> 3;
+    const uint32_t dst0 = r0 * 128 + ((piece ^ (r0 & 7)) << 4);
     GlRing<S> at;
-    int64_t filled = 0;
     bool ok = true;
     for (int t = t0; t < tiles && ok; t += stride) {
         const GlTile x = gl_tile<MODE, BN, SPLIT>(a, t, rank, ranks);
         if (x.c0 == x.c1) continue;
-        int rows[4];
-        int boxes_a = 0, boxes_b = 0;
-        if (MODE == kModeDw) {
-            boxes_a = x.row0 + 64 < a.N ? 2 : 1;  // a block wholly outside is not needed: its rows of D are never read
-            boxes_b = min(BN / 64, (a.cols - x.col0 + 63) / 64);
-        } else {
+        constexpr int kRows = MODE == kModeDw ? 4 : 8;
+        int rows[kRows];
+        auto rows_of = [&](int i0, int(&r)[kRows]) {  // rows i0 + r0 + 16 i of the tile's or bucket's list; -1 behind its end
 #pragma unroll
-            for (int j = 0; j < 4; ++j) rows[j] = 4 * lane + j < x.count ? __ldg(a.plan.order + x.first + 4 * lane + j) : a.T;
-            boxes_b = min(BN / 64, (a.cols - x.col0 + 63) / 64);
-        }
-        auto bucket_rows = [&](int c, int(&r)[4]) {  // dw: the four rows of this lane in chunk c
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = c * kGlK + 4 * (lane & 15) + j;
-                r[j] = i < x.count ? __ldg(a.plan.order + x.first + i) : a.T;
+            for (int i = 0; i < kRows; ++i) {
+                const int k = i0 + r0 + 16 * i;
+                r[i] = k < x.count ? __ldg(a.plan.order + x.first + k) : -1;
             }
         };
-        if (MODE == kModeDw) bucket_rows(x.c0, rows);
+        rows_of(MODE == kModeDw ? x.c0 * kGlK : 0, rows);
         for (int c = x.c0; c < x.c1; ++c) {
-            int ahead[4];
-            if (MODE == kModeDw && c + 1 < x.c1) bucket_rows(c + 1, ahead);  // on their way while this stage is awaited
+            int ahead[kRows];
+            if (MODE == kModeDw) rows_of((c + 1) * kGlK, ahead);  // on their way while this stage is awaited
             if (lane == 0) ok = mbar_wait_timed(empty + at.stage, at.phase ^ 1u);
             ok = __shfl_sync(kFullMask, ok, 0);
             if (!ok) break;
             const uint32_t sa = ring + at.stage * gl_stage_bytes(BN), sb = sa + kGlABytes;
             uint64_t* bar = full + at.stage;
             if (MODE == kModeDw) {
-                const int quads = 4 * gl_steps<MODE>(a, x, c);
-                if (lane == 0) mbar_expect_tx(bar, (boxes_a + boxes_b) * quads * 512);
-                __syncwarp();
-                const int q = lane & 15;
-                if (q < quads)
-                    for (int b = lane >> 4; b < boxes_a + boxes_b; b += 2) {
-                        const bool is_a = b < boxes_a;
-                        const int i = is_a ? b : b - boxes_a;
-                        tma_gather4((is_a ? sa : sb) + i * kGlBoxBytes + q * 512, is_a ? map_a : map_b,
-                                    (is_a ? x.row0 : x.col0) + i * 64, rows[0], rows[1], rows[2], rows[3], bar);
+                const int n = 16 * gl_steps<MODE>(a, x, c);
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) {
+                    if (16 * i >= n) break;
+                    const bool live = rows[i] >= 0;
+                    const unsigned char* pa = a.rows_a + (live ? rows[i] * a.pitch_a : 0);
+                    const unsigned char* pb = a.rows_b + (live ? rows[i] * a.pitch_b : 0);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int col = x.row0 + b * 64 + piece * 8;
+                        if (x.row0 + b * 64 < a.N) cp_async16_n(sa + b * kGlBoxBytes + dst0 + i * 2048, pa, col, live ? a.N - col : 0);
                     }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) rows[j] = ahead[j];
-            } else {
-                const int b_bytes = MODE == kModeFwd ? BN * 128 : boxes_b * kGlBoxBytes;
-                if (lane == 0) mbar_expect_tx(bar, ((x.count + 3) >> 2) * 512 + b_bytes);
-                __syncwarp();
-                if (4 * lane < x.count) tma_gather4(sa + lane * 512, map_a, c * kGlK, rows[0], rows[1], rows[2], rows[3], bar);
-                if (MODE == kModeFwd) {
-                    if (lane == 0) tma_tile_3d(sb, map_b, c * kGlK, x.col0, x.bucket, bar);
-                } else if (lane < boxes_b) {
-                    tma_tile_3d(sb + lane * kGlBoxBytes, map_b, x.col0 + lane * 64, c * kGlK, x.bucket, bar);
+                    for (int b = 0; b < BN / 64; ++b) {
+                        const int col = x.col0 + b * 64 + piece * 8;
+                        if (x.col0 + b * 64 < a.cols) cp_async16_n(sb + b * kGlBoxBytes + dst0 + i * 2048, pb, col, live ? a.cols - col : 0);
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) rows[i] = ahead[i];
+            } else {
+                if (j < (MODE == kModeFwd ? 1 : BN / 64)) {  // w comes as whole boxes
+                    if (MODE == kModeFwd) {
+                        mbar_expect_tx(bar, BN * 128);
+                        tma_tile_3d(sb, map_b, c * kGlK, x.col0, x.bucket, bar);
+                    } else {
+                        const int boxes = min(BN / 64, (a.cols - x.col0 + 63) >> 6);
+                        if (j == 0) mbar_expect_tx(bar, boxes * kGlBoxBytes);
+                        if (j < boxes) tma_tile_3d(sb + j * kGlBoxBytes, map_b, x.col0 + j * 64, c * kGlK, x.bucket, bar);
+                    }
+                }
+                const int col = c * kGlK + piece * 8;
+#pragma unroll
+                for (int i = 0; i < kRows; ++i)
+                    if (rows[i] >= 0) cp_async16_n(sa + dst0 + i * 2048, a.rows_a + rows[i] * a.pitch_a, col, a.red - col);
             }
-            __syncwarp();
-            ++filled;
+            cp_async_arrive(bar);
             at.next();
         }
     }
-    if (!ok && lane == 0) {  // copies in flight land before the CTA leaves
-        for (int i = 0; i < S && i < filled; ++i) {
-            const int64_t n = filled - 1 - i;
-            mbar_wait_timed(full + n % S, (unsigned)((n / S) & 1));
-        }
-    }
+    if (!ok) cp_async_wait<0>();  // copies in flight land before the CTA leaves; w's boxes are older than the wait that ran out
     return ok;
 }
 
@@ -298,6 +301,7 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
         for (int c = x.c0; c < x.c1; ++c) {
             ok = mbar_wait_timed(full + at.stage, at.phase);
             if (!ok) break;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the gathered rows were written by ordinary copies
             tc_fence_after();
             const uint32_t sa = ring + at.stage * gl_stage_bytes(BN);
             const uint64_t da = umma_desc_sw128(sa, kGlBoxBytes), db = umma_desc_sw128(sa + kGlABytes, kGlBoxBytes);
@@ -326,7 +330,7 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
 template <int BN, bool SPLIT>
 __device__ __forceinline__ bool gl_sums_role(const GlArgs& a, const unsigned char* ring, uint64_t* full, uint64_t* empty,
                                              float* s_sums, int t0, int stride, int tiles, int rank, int ranks) {
-    const int n = threadIdx.x - 192, lane = threadIdx.x & 31;
+    const int n = threadIdx.x - 288, lane = threadIdx.x & 31;
     GlRing<gl_stages(BN)> at;
     bool ok = true;
     for (int t = t0; t < tiles && ok; t += stride) {
@@ -362,7 +366,7 @@ __device__ __forceinline__ bool gl_sums_role(const GlArgs& a, const unsigned cha
 
 template <int MODE, int BN, bool SPLIT>
 __global__ void __launch_bounds__(gl_threads(MODE), 1)
-    k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GlArgs a) {
+    k_grouped(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GlArgs a) {
     constexpr int S = gl_stages(BN);
     constexpr uint32_t kTmemCols = 2 * BN;
     constexpr int kPartPitch = BN + 4;  // floats per row of a partial tile
@@ -393,7 +397,7 @@ __global__ void __launch_bounds__(gl_threads(MODE), 1)
 
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(full + s, 1);
+            mbar_init(full + s, MODE == kModeDw ? 128 : 129);  // the copying threads, and the boxes of w
             mbar_init(empty + s, MODE == kModeDw ? 5 : 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -402,21 +406,20 @@ __global__ void __launch_bounds__(gl_threads(MODE), 1)
         }
         mbar_init(drained, 1);
         fence_barrier_init();
-        prefetch_map(&map_a);
-        prefetch_map(&map_b);
+        if (MODE != kModeDw) prefetch_map(&map_b);
     }
-    if (warp == 1) tmem_alloc(s_tmem, kTmemCols);
+    if (warp == 4) tmem_alloc(s_tmem, kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
 
     bool ok = true;
-    if (warp == 0) {
-        ok = gl_copy_role<MODE, BN, SPLIT>(a, &map_a, &map_b, ring, full, empty, t0, stride, tiles, rank, ranks);
-    } else if (warp == 1) {
+    if (warp < 4) {
+        ok = gl_copy_role<MODE, BN, SPLIT>(a, &map_b, ring, full, empty, t0, stride, tiles, rank, ranks);
+    } else if (warp == 4) {
         if (lane == 0) ok = gl_issue_role<MODE, BN, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
-    } else if (warp < 6) {
+    } else if (warp < 9) {
         const int q = warp & 3;  // the quarter of tensor memory's lanes that this warp may read
         float* my_bias = s_bias + q * BN;
         int acc = 0;
@@ -478,7 +481,7 @@ __global__ void __launch_bounds__(gl_threads(MODE), 1)
     if (SPLIT) {
         __syncthreads();  // nobody reads the ring any more: the partial tile takes its place
         const GlTile x = gl_tile<MODE, BN, SPLIT>(a, t0, rank, ranks);
-        if (warp >= 2 && warp < 6) {
+        if (warp >= 5 && warp < 9) {
             const int q = warp & 3;
             float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * kPartPitch;
 #pragma unroll 1
@@ -550,12 +553,12 @@ __global__ void __launch_bounds__(gl_threads(MODE), 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) tmem_free(tmem, kTmemCols);
+    if (warp == 4) tmem_free(tmem, kTmemCols);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 template <int MODE, int BN, bool SPLIT>
-int gl_launch(const CUtensorMap& ma, const CUtensorMap& mb, const GlArgs& a, int64_t tiles, int ranks, cudaStream_t s) {
+int gl_launch(const CUtensorMap& mb, const GlArgs& a, int64_t tiles, int ranks, cudaStream_t s) {
     auto kernel = k_grouped<MODE, BN, SPLIT>;
     static bool opted[64] = {};  // more than 48 KB of dynamic shared memory needs the opt-in, once per device
     int dev = 0;
@@ -578,7 +581,7 @@ int gl_launch(const CUtensorMap& ma, const CUtensorMap& mb, const GlArgs& a, int
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
     }
-    NNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, a));
+    NNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mb, a));
     note_launches(1);
     return NNUE_OK;
 }
@@ -600,32 +603,26 @@ static GlShape gl_shape(int64_t row_tiles, int64_t cols, int64_t chunks, int nar
 }
 
 template <int MODE>
-int gl_run(const CUtensorMap& ma, const CUtensorMap& mb, GlArgs& a, int64_t tile_rows, GlShape shape, cudaStream_t s) {
+int gl_run(const CUtensorMap& mb, GlArgs& a, int64_t tile_rows, GlShape shape, cudaStream_t s) {
     a.col_tiles = (a.cols + shape.bn - 1) / shape.bn;
     a.idesc = umma_idesc(a.idesc, (uint32_t)shape.bn, MODE == kModeDw, MODE != kModeFwd);
     const int64_t tiles = tile_rows * a.col_tiles;
     NNUE_REQUIRE(tiles * 8 < 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "grouped linear: too many tiles");
     if (MODE == kModeFwd && shape.bn == 32)
-        return shape.ranks > 1 ? gl_launch<MODE, MODE == kModeFwd ? 32 : 64, true>(ma, mb, a, tiles, shape.ranks, s)
-                               : gl_launch<MODE, MODE == kModeFwd ? 32 : 64, false>(ma, mb, a, tiles, 1, s);
+        return shape.ranks > 1 ? gl_launch<MODE, MODE == kModeFwd ? 32 : 64, true>(mb, a, tiles, shape.ranks, s)
+                               : gl_launch<MODE, MODE == kModeFwd ? 32 : 64, false>(mb, a, tiles, 1, s);
     if (shape.bn == 64)
-        return shape.ranks > 1 ? gl_launch<MODE, 64, true>(ma, mb, a, tiles, shape.ranks, s)
-                               : gl_launch<MODE, 64, false>(ma, mb, a, tiles, 1, s);
+        return shape.ranks > 1 ? gl_launch<MODE, 64, true>(mb, a, tiles, shape.ranks, s)
+                               : gl_launch<MODE, 64, false>(mb, a, tiles, 1, s);
     if (shape.bn == 128)
-        return shape.ranks > 1 ? gl_launch<MODE, 128, true>(ma, mb, a, tiles, shape.ranks, s)
-                               : gl_launch<MODE, 128, false>(ma, mb, a, tiles, 1, s);
-    return shape.ranks > 1 ? gl_launch<MODE, 256, true>(ma, mb, a, tiles, shape.ranks, s)
-                           : gl_launch<MODE, 256, false>(ma, mb, a, tiles, 1, s);
+        return shape.ranks > 1 ? gl_launch<MODE, 128, true>(mb, a, tiles, shape.ranks, s)
+                               : gl_launch<MODE, 128, false>(mb, a, tiles, 1, s);
+    return shape.ranks > 1 ? gl_launch<MODE, 256, true>(mb, a, tiles, shape.ranks, s)
+                           : gl_launch<MODE, 256, false>(mb, a, tiles, 1, s);
 }
 
 static CUtensorMapDataType map_type(int32_t type) {
     return type == NNUE_T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-}
-// [rows, cols] read four rows at a time, 64 columns each
-static int rows_map(CUtensorMap* map, const void* p, int64_t ld, int64_t rows, int64_t cols, int32_t type) {
-    const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)ld * 2};
-    const uint32_t box[2] = {64, 1};
-    return encode_map(map, map_type(type), 2, p, dims, strides, box);
 }
 // [E, N, K] read in boxes of 64 columns and `high` rows of one bucket
 static int weight_map(CUtensorMap* map, const void* p, int64_t ld, int64_t E, int64_t N, int64_t K, int high, int32_t type) {
@@ -730,10 +727,11 @@ extern "C" int nnue_grouped_linear_fwd(const void* x, int64_t ldx, const void* w
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("grouped_fwd", s);
     const GlShape shape = gl_shape(expected_row_tiles(T, E), N, (K + kGlK - 1) / kGlK, 32);
-    CUtensorMap ma, mb;
-    if (int st = rows_map(&ma, x, ldx, T, K, type)) return st;
+    a.rows_a = static_cast<const unsigned char*>(x);
+    a.pitch_a = ldx * 2;
+    CUtensorMap mb;
     if (int st = weight_map(&mb, w, ldw, E, N, K, shape.bn, type)) return st;
-    return gl_run<kModeFwd>(ma, mb, a, group_max_tiles(T, E), shape, s);
+    return gl_run<kModeFwd>(mb, a, group_max_tiles(T, E), shape, s);
 }
 
 extern "C" int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, const void* w, int64_t ldw, const void* plan, void* dx,
@@ -749,10 +747,11 @@ extern "C" int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, const
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("grouped_dx", s);
     const GlShape shape = gl_shape(expected_row_tiles(T, E), K, (N + kGlK - 1) / kGlK, 64);
-    CUtensorMap ma, mb;
-    if (int st = rows_map(&ma, dy, lddy, T, N, type)) return st;
+    a.rows_a = static_cast<const unsigned char*>(dy);
+    a.pitch_a = lddy * 2;
+    CUtensorMap mb;
     if (int st = weight_map(&mb, w, ldw, E, N, K, 64, type)) return st;
-    return gl_run<kModeDx>(ma, mb, a, group_max_tiles(T, E), shape, s);
+    return gl_run<kModeDx>(mb, a, group_max_tiles(T, E), shape, s);
 }
 
 extern "C" int nnue_grouped_linear_bwd_weight(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* plan, void* dw,
@@ -775,13 +774,10 @@ extern "C" int nnue_grouped_linear_bwd_weight(const void* dy, int64_t lddy, cons
     ProfScope prof("grouped_dw", s);
     const int64_t row_tiles = (int64_t)E * a.row_tiles, mean = (T + E - 1) / E;
     const GlShape shape = gl_shape(row_tiles, K, (mean + kGlK - 1) / kGlK, 64);
-    CUtensorMap ma, mb;
-    if (T > 0) {
-        if (int st = rows_map(&ma, dy, lddy, T, N, type)) return st;
-        if (int st = rows_map(&mb, x, ldx, T, K, type)) return st;
-    } else {  // no row is read: any valid map
-        if (int st = rows_map(&ma, dw, 64, 1, 1, type)) return st;
-        mb = ma;
-    }
-    return gl_run<kModeDw>(ma, mb, a, row_tiles, shape, s);
+    a.rows_a = static_cast<const unsigned char*>(dy);
+    a.pitch_a = lddy * 2;
+    a.rows_b = static_cast<const unsigned char*>(x);
+    a.pitch_b = ldx * 2;
+    const CUtensorMap none = {};  // both operands are gathered
+    return gl_run<kModeDw>(none, a, row_tiles, shape, s);
 }

@@ -66,13 +66,15 @@ __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// Columns [x, x + box) of four rows of a 2-D map whose box is one row high; a row outside the map reads as zeros.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], "
-        "[%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
-        : "memory");
+// 16 bytes to shared memory: `left` 16-bit elements from column `col` of a row on, zeros behind them (none: nothing is read)
+__device__ __forceinline__ void cp_async16_n(uint32_t dst, const unsigned char* row, int col, int left) {
+    const int n = left >= 8 ? 16 : left > 0 ? 2 * left : 0;
+    const unsigned char* src = n ? row + (int64_t)col * 2 : row;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+// arrives on `bar` when every copy this thread has started so far has landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Matrix descriptor of an operand in 128-byte-swizzled shared memory (1024-byte aligned groups of 8 rows of 128 bytes).
