@@ -742,28 +742,49 @@ int nnue_pack_rows(const void* src, int32_t src_type, int64_t lds, void* dst,
                    int32_t dst_type, int64_t ldd, int64_t rows, int64_t cols,
                    void* stream);
 
+/* The batch's rows laid out by bucket: 16-bit numbers, rows of cols numbers
+ * rounded up to a multiple of 8, every bucket from a multiple of 64 rows on;
+ * what lies between a bucket's last row and the next multiple is zero.  src [T,
+ * cols] (pitch ld) of `type` or any other float type (one rounding); dst of
+ * nnue_group_rows_bytes bytes, 16-byte aligned.  Rows without a bucket are left
+ * out.  sums: NULL, or nnue_group_sums_bytes bytes that receive the sums of the
+ * columns of each tile of 128 rows, for nnue_grouped_linear_bwd_weight. */
+size_t nnue_group_rows_bytes(int64_t T, int64_t cols, int32_t E);
+size_t nnue_group_sums_bytes(int64_t T, int64_t cols, int32_t E);
+int nnue_group_rows(const void* src, int32_t src_type, int64_t ld,
+                    const void* plan, void* dst, int32_t type, float* sums,
+                    int64_t T, int64_t cols, int32_t E, void* stream);
+/* out[b, c] (any float type) = sum over the rows of bucket b, from such sums. */
+int nnue_group_sums(const float* sums, const void* plan, void* out,
+                    int32_t type, int64_t T, int64_t cols, int32_t E,
+                    void* stream);
+
 /* y[p, n]  = sum_k x[p, k] w[b, n, k] + bias[b, n],  b = bucket of row p
  * dx[p, k] = sum_n dy[p, n] w[b, n, k]
  * dw[b, n, k] = sum_{p of b} dy[p, n] x[p, k],  dbias[b, n] = sum_{p of b} dy[p, n]
- * x [T, K], w [E, N, K], dy [T, N] of `type` (BF16 or F16), rows at pitches ldx,
- * ldw, lddy (elements) that are multiples of 16 bytes; bias [E, N] of any of the
- * three float types, may be NULL; y [T, N], dx [T, K] and dw [E, N, K] contiguous,
- * y and dw of `type` or F32, dx of `type`, dbias [E, N] of any float type, may be
- * NULL.  Sums are fp32, rounded once.  Rows without a bucket get zeros in y and
- * dx, whatever they hold; a bucket without rows gets zeros in dw and dbias.  Sums
- * run in an order that the sizes alone fix: results are reproducible.  T = 0 is
- * allowed.  `plan`: nnue_group_plan's, of the same T and E. */
-int nnue_grouped_linear_fwd(const void* x, int64_t ldx, const void* w,
-                            int64_t ldw, const void* bias, int32_t bias_type,
-                            const void* plan, void* y, int32_t y_type, int64_t T,
-                            int64_t K, int64_t N, int32_t E, int32_t type,
-                            void* stream);
-int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, const void* w,
-                                  int64_t ldw, const void* plan, void* dx,
-                                  int64_t T, int64_t K, int64_t N, int32_t E,
-                                  int32_t type, void* stream);
-int nnue_grouped_linear_bwd_weight(const void* dy, int64_t lddy, const void* x,
-                                   int64_t ldx, const void* plan, void* dw,
+ * x [T, K], w [E, N, K], dy [T, N] of `type` (BF16 or F16); w at a pitch ldw
+ * (elements) that is a multiple of 16 bytes.  x and dy: with `laid`, as
+ * nnue_group_rows leaves them (ldx, lddy are not looked at); else in the batch's
+ * order at such a pitch, which suits a few rows per bucket (they are gathered).
+ * bwd_weight takes both laid out, and dy's sums where dbias is wanted.
+ * bias [E, N] of any of the three float types, may be NULL; y [T, N], dx [T, K] and
+ * dw [E, N, K] contiguous, y and dw of `type` or F32, dx of `type`, dbias [E, N] of
+ * any float type, may be NULL.  Sums are fp32, rounded once.  Rows without a
+ * bucket get zeros in y and dx, whatever they hold; a bucket without rows gets
+ * zeros in dw and dbias.  Sums run in an order that the sizes alone fix: results
+ * are reproducible.  T = 0 is allowed.  `plan`: nnue_group_plan's, of the same T
+ * and E. */
+int nnue_grouped_linear_fwd(const void* x, int64_t ldx, int32_t laid,
+                            const void* w, int64_t ldw, const void* bias,
+                            int32_t bias_type, const void* plan, void* y,
+                            int32_t y_type, int64_t T, int64_t K, int64_t N,
+                            int32_t E, int32_t type, void* stream);
+int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, int32_t laid,
+                                  const void* w, int64_t ldw, const void* plan,
+                                  void* dx, int64_t T, int64_t K, int64_t N,
+                                  int32_t E, int32_t type, void* stream);
+int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_sums,
+                                   const void* x, const void* plan, void* dw,
                                    int32_t dw_type, void* dbias,
                                    int32_t dbias_type, int64_t T, int64_t K,
                                    int64_t N, int32_t E, int32_t type,

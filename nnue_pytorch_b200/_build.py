@@ -38,6 +38,7 @@ SOURCES = [
     "batch_build.cu",
     "sf_loss.cu",
     "group_plan.cu",
+    "group_rows.cu",
     "grouped_linear.cu",
     "fp8_blocks.cu",
     "fp8_linear.cu",

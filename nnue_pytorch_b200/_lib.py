@@ -233,15 +233,16 @@ PROTOTYPES = {
     "nnue_group_plan_bytes": (_SZ, [_I64, _I32]),
     "nnue_group_plan": (C.c_int, [_P, _I32, _I64, _I32, _P, _SZ, _P]),
     "nnue_pack_rows": (C.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _P]),
+    "nnue_group_rows_bytes": (_SZ, [_I64, _I64, _I32]),
+    "nnue_group_sums_bytes": (_SZ, [_I64, _I64, _I32]),
+    "nnue_group_rows": (C.c_int, [_P, _I32, _I64, _P, _P, _I32, _P, _I64, _I64, _I32, _P]),
+    "nnue_group_sums": (C.c_int, [_P, _P, _P, _I32, _I64, _I64, _I32, _P]),
     "nnue_grouped_linear_fwd": (
         C.c_int,
-        [_P, _I64, _P, _I64, _P, _I32, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P],
+        [_P, _I64, _I32, _P, _I64, _P, _I32, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P],
     ),
-    "nnue_grouped_linear_bwd_input": (C.c_int, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P]),
-    "nnue_grouped_linear_bwd_weight": (
-        C.c_int,
-        [_P, _I64, _P, _I64, _P, _P, _I32, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P],
-    ),
+    "nnue_grouped_linear_bwd_input": (C.c_int, [_P, _I64, _I32, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P]),
+    "nnue_grouped_linear_bwd_weight": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P]),
     "nnue_fp8_quantize_rows": (C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I64, _I64, _I32, _P]),
     "nnue_fp8_quantize_tiles": (C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I32, _I64, _I64, _I32, _P]),
     "nnue_fp8_linear_fwd": (

@@ -76,86 +76,96 @@ __device__ __forceinline__ void group_fill(const Id* bucket, int64_t lo, int64_t
     }
 }
 
-// exclusive scan over the block of one pair of values per thread; the totals go to `total`
-__device__ __forceinline__ int2 block_scan2(int2 v, int2* s_warp, int2* total) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int2 inc = v;
+// exclusive scan over the block of four values per thread; the totals go to `total`
+__device__ __forceinline__ int4 add4(int4 a, int4 b) { return make_int4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+__device__ __forceinline__ int4 warp_scan4(int4 v) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int x = __shfl_up_sync(kFullMask, inc.x, d), y = __shfl_up_sync(kFullMask, inc.y, d);
-        if (lane >= d) { inc.x += x; inc.y += y; }
+        const int4 u = make_int4(__shfl_up_sync(kFullMask, v.x, d), __shfl_up_sync(kFullMask, v.y, d),
+                                 __shfl_up_sync(kFullMask, v.z, d), __shfl_up_sync(kFullMask, v.w, d));
+        if (lane >= d) v = add4(v, u);
     }
+    return v;
+}
+__device__ __forceinline__ int4 block_scan4(int4 v, int4* s_warp, int4* total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int4 inc = warp_scan4(v);
     __syncthreads();
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    if (warp == 0) {
-        int2 w = s_warp[lane];
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int x = __shfl_up_sync(kFullMask, w.x, d), y = __shfl_up_sync(kFullMask, w.y, d);
-            if (lane >= d) { w.x += x; w.y += y; }
-        }
-        s_warp[lane] = w;
-    }
+    if (warp == 0) s_warp[lane] = warp_scan4(s_warp[lane]);
     __syncthreads();
-    const int2 before = warp ? s_warp[warp - 1] : make_int2(0, 0);
+    const int4 before = warp ? s_warp[warp - 1] : make_int4(0, 0, 0, 0);
     *total = s_warp[kGpWarps - 1];
-    return make_int2(before.x + inc.x - v.x, before.y + inc.y - v.y);
+    return make_int4(before.x + inc.x - v.x, before.y + inc.y - v.y, before.z + inc.z - v.z, before.w + inc.w - v.w);
 }
 
-// Totals of the bins (s_total) to the plan's offsets and tile list; s_base[bin] = first place, s_tile[bin] = first tile.
-__device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_total, int32_t* s_base, int32_t* s_tile,
-                                            int2* s_warp, int32_t* plan) {
+// Totals of the bins (s_total) to the plan's offsets, places and tile lists.  s_at[bin] = first place in the order, first
+// tile, first pair, first place among rows laid out by bucket.
+__device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_total, int4* s_at, int4* s_warp, int32_t* plan) {
     const int bins = E + 1;
-    int2 carry = make_int2(0, 0);
+    int4 carry = make_int4(0, 0, 0, 0);
     for (int b0 = 0; b0 < bins; b0 += kGpThreads) {
         const int b = b0 + threadIdx.x;
         const int n = b < bins ? s_total[b] : 0;
-        int2 total;
-        const int2 ex = block_scan2(make_int2(n, (n + kGroupRows - 1) / kGroupRows), s_warp, &total);
+        int4 total;
+        const int4 mine = make_int4(n, (n + kGroupRows - 1) / kGroupRows, (n + kGroupPairRows - 1) / kGroupPairRows,
+                                    b < E ? (n + kGroupAlign - 1) / kGroupAlign * kGroupAlign : 0);
+        const int4 at = add4(carry, block_scan4(mine, s_warp, &total));
         if (b < bins) {
-            s_base[b] = carry.x + ex.x;
-            s_tile[b] = carry.y + ex.y;
-            plan[group_offsets_at() + b] = carry.x + ex.x;
+            s_at[b] = at;
+            plan[group_offsets_at() + b] = at.x;
+            plan[group_places_at(T, E) + b] = at.w;
+            plan[group_first_at(T, E) + b] = at.y;
         }
-        carry.x += total.x;
-        carry.y += total.y;
+        carry = add4(carry, total);
     }
     if (threadIdx.x == 0) {
-        s_tile[bins] = carry.y;
+        s_at[bins] = carry;
         plan[0] = carry.y;
+        plan[1] = carry.z;
         plan[group_offsets_at() + bins] = (int32_t)T;
     }
     __syncthreads();
-    int4* tiles = reinterpret_cast<int4*>(plan + group_tiles_at(T, E));
-    for (int t = threadIdx.x; t < s_tile[bins]; t += kGpThreads) {
-        int lo = 0, hi = bins - 1;  // the last bin whose first tile is not behind t; empty bins share a first tile
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_tile[mid] <= t) lo = mid;
-            else hi = mid - 1;
+    for (int pairs = 0; pairs < 2; ++pairs) {
+        int4* tiles = reinterpret_cast<int4*>(plan + (pairs ? group_pairs_at(T, E) : group_tiles_at(T, E)));
+        const int rows = pairs ? kGroupPairRows : kGroupRows;
+        for (int t = threadIdx.x; t < (pairs ? carry.z : carry.y); t += kGpThreads) {
+            int lo = 0, hi = bins - 1;  // the last bin whose first tile is not behind t; empty bins share a first tile
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if ((pairs ? s_at[mid].z : s_at[mid].y) <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int4 b = s_at[lo];
+            const int in = (t - (pairs ? b.z : b.y)) * rows;
+            tiles[t] = make_int4(lo, b.x + in, min(rows, s_total[lo] - in), b.w + in);
         }
-        const int at = (t - s_tile[lo]) * kGroupRows;
-        tiles[t] = make_int4(lo, s_base[lo] + at, min(kGroupRows, s_total[lo] - at), 0);
     }
 }
 
-constexpr size_t group_smem_bytes(int bins) { return sizeof(int32_t) * ((size_t)bins * kGpWarps + 3 * (size_t)bins + 2); }
+// shared memory: s_at [bins + 1] int4, counters per warp [bins][kGpWarps] (not in the scan), totals [bins]
+constexpr size_t group_smem_bytes(int bins, bool counters) {
+    return sizeof(int4) * (bins + 1) + sizeof(int32_t) * ((counters ? (size_t)bins * kGpWarps : 0) + bins);
+}
 
 template <typename Id>
 __global__ void __launch_bounds__(kGpThreads)
     k_group_single(const Id* __restrict__ bucket, int64_t T, int E, int32_t* __restrict__ plan, unsigned long long* status) {
-    extern __shared__ int32_t s_hist[];
+    extern __shared__ int4 s_at[];
     const int bins = E + 1;
+    int32_t* s_hist = reinterpret_cast<int32_t*>(s_at + bins + 1);
     int32_t* s_total = s_hist + bins * kGpWarps;
-    int32_t* s_base = s_total + bins;
-    int32_t* s_tile = s_base + bins;  // [bins + 1]
-    __shared__ int2 s_warp[kGpWarps];
+    __shared__ int4 s_warp[kGpWarps];
     group_histogram(bucket, 0, T, bins, s_hist, status);
     for (int b = threadIdx.x; b < bins; b += kGpThreads) s_total[b] = group_scan_warps(s_hist, bins, b);
     __syncthreads();
-    group_tiles(T, E, s_total, s_base, s_tile, s_warp, plan);
-    group_fill(bucket, 0, T, bins, s_hist, s_base, plan + group_order_at(E));
+    group_tiles(T, E, s_total, s_at, s_warp, plan);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kGpThreads) s_total[b] = s_at[b].x;  // from here on: first places
+    __syncthreads();
+    group_fill(bucket, 0, T, bins, s_hist, s_total, plan + group_order_at(E));
 }
 
 // long form, 1: counts[bin][block]
@@ -173,11 +183,10 @@ __global__ void __launch_bounds__(kGpThreads)
 // long form, 2: counts[bin][block] becomes the number of rows of `bin` in the blocks before, and the plan's head
 __global__ void __launch_bounds__(kGpThreads)
     k_group_scan(int64_t T, int E, int blocks, int32_t* __restrict__ counts, int32_t* __restrict__ plan) {
-    extern __shared__ int32_t s_total[];
+    extern __shared__ int4 s_at[];
     const int bins = E + 1;
-    int32_t* s_base = s_total + bins;
-    int32_t* s_tile = s_base + bins;
-    __shared__ int2 s_warp[kGpWarps];
+    int32_t* s_total = reinterpret_cast<int32_t*>(s_at + bins + 1);
+    __shared__ int4 s_warp[kGpWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int b = warp; b < bins; b += kGpWarps) {
         int run = 0;
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(kGpThreads)
         if (lane == 0) s_total[b] = run;
     }
     __syncthreads();
-    group_tiles(T, E, s_total, s_base, s_tile, s_warp, plan);
+    group_tiles(T, E, s_total, s_at, s_warp, plan);
 }
 
 // long form, 3: rows to their places
@@ -221,12 +230,12 @@ inline int64_t group_blocks(int64_t T) { return T <= kSingleRows ? 0 : (T + kBlo
 template <typename Id>
 int launch_plan(const Id* bucket, int64_t T, int32_t E, int32_t* plan, unsigned long long* status, cudaStream_t s) {
     const int bins = E + 1;
-    const size_t smem = group_smem_bytes(bins);
+    const size_t smem = group_smem_bytes(bins, true);
     static bool opted[64] = {};  // more than 48 KB of dynamic shared memory needs the opt-in, once per device
     int dev = 0;
     NNUE_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !opted[dev]) {
-        const int most = (int)group_smem_bytes(kMaxGroups + 1);
+        const int most = (int)group_smem_bytes(kMaxGroups + 1, true);
         NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_single<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_count<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_fill<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
@@ -239,7 +248,7 @@ int launch_plan(const Id* bucket, int64_t T, int32_t E, int32_t* plan, unsigned 
     } else {
         int32_t* counts = plan + group_counts_at(T, E);
         k_group_count<Id><<<(unsigned)blocks, kGpThreads, smem, s>>>(bucket, T, E, counts, status);
-        k_group_scan<<<1, kGpThreads, sizeof(int32_t) * (3 * bins + 2), s>>>(T, E, (int)blocks, counts, plan);
+        k_group_scan<<<1, kGpThreads, group_smem_bytes(bins, false), s>>>(T, E, (int)blocks, counts, plan);
         k_group_fill<Id><<<(unsigned)blocks, kGpThreads, smem, s>>>(bucket, T, E, counts, plan);
         note_launches(3);
     }

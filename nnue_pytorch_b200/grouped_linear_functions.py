@@ -99,6 +99,23 @@ def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev) -> tuple[torch.Tenso
     return out, pitch
 
 
+def _laid_out(t: torch.Tensor, dtype: torch.dtype, plan_buffer, E: int, lib, dev, sums: bool = False):
+    """(t laid out by bucket as `dtype` (`nnue_group_rows`), the sums of its columns per tile or None)."""
+    T, cols = t.shape
+    if cols > 1 and t.stride(1) != 1 or t.stride(0) < cols:
+        t = t.contiguous()
+    out = torch.empty(lib.nnue_group_rows_bytes(T, cols, E), dtype=torch.uint8, device=dev)
+    part = torch.empty(lib.nnue_group_sums_bytes(T, cols, E) // 4, dtype=torch.float32, device=dev) if sums else None
+    st = lib.nnue_group_rows(_ptr(t), TYPES[t.dtype], t.stride(0), _ptr(plan_buffer), _ptr(out), TYPES[dtype], _ptr(part), T, cols,
+                             E, _stream(dev))
+    _lib.check(st, "nnue_group_rows")
+    return out, part
+
+
+# Up to this many rows per bucket the products gather them as they lie; beyond it they are laid out by bucket first.
+GATHERED_ROWS = 16
+
+
 class GroupedLinearFunction(autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, plan, out_dtype=None):
@@ -120,16 +137,21 @@ class GroupedLinearFunction(autograd.Function):
             assert bias.dtype in (dtype, torch.float32) and bias.numel() == E * N
         lib = _lib.load()
         y = torch.empty(T, N, dtype=out_dtype, device=dev)
+        # the weight gradient reads the rows laid out by bucket, and so does the forward unless they are few
+        laid = ctx.needs_input_grad[1] or T > GATHERED_ROWS * E
         with _on(dev), _span("grouped_linear_fwd", dev):
-            xr, ldx = _pitched(x.detach(), dtype, lib, dev)
+            if laid:
+                xr, ldx = _laid_out(x.detach(), dtype, plan.buffer, E, lib, dev)[0], 0
+            else:
+                xr, ldx = _pitched(x.detach(), dtype, lib, dev)
             wr, ldw = _pitched(w2, dtype, lib, dev)
             b = None if bias is None else bias.detach().contiguous()
             st = lib.nnue_grouped_linear_fwd(
-                _ptr(xr), ldx, _ptr(wr), ldw, _ptr(b), 0 if b is None else TYPES[b.dtype], _ptr(plan.buffer), _ptr(y),
+                _ptr(xr), ldx, laid, _ptr(wr), ldw, _ptr(b), 0 if b is None else TYPES[b.dtype], _ptr(plan.buffer), _ptr(y),
                 TYPES[out_dtype], T, K, N, E, TYPES[dtype], _stream(dev))
         _lib.check(st, "nnue_grouped_linear_fwd")
-        ctx.save_for_backward(xr, wr, plan.buffer)
-        ctx.dims = (T, K, N, E, ldx, ldw)
+        ctx.save_for_backward(xr if ctx.needs_input_grad[1] else None, wr if ctx.needs_input_grad[0] else None, plan.buffer)
+        ctx.dims = (T, K, N, E, ldw)
         ctx.dtype, ctx.w_like, ctx.b_like = dtype, (weight.dtype, weight.shape), None if bias is None else (bias.dtype, bias.shape)
         return y
 
@@ -137,27 +159,33 @@ class GroupedLinearFunction(autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, plan = ctx.saved_tensors
-        T, K, N, E, ldx, ldw = ctx.dims
-        dev, dtype = x.device, ctx.dtype
+        T, K, N, E, ldw = ctx.dims
+        dev, dtype = dy.device, ctx.dtype
         lib = _lib.load()
+        need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         dx = dw = db = None
         with _on(dev), _span("grouped_linear_bwd", dev):
             s = _stream(dev)
-            dyr, lddy = _pitched(dy, dtype, lib, dev)
-            if ctx.needs_input_grad[0]:
+            if need_w or need_b or T > GATHERED_ROWS * E:
+                dyr, part = _laid_out(dy, dtype, plan, E, lib, dev, sums=need_b)
+                laid, lddy = 1, 0
+            else:
+                dyr, lddy = _pitched(dy, dtype, lib, dev)
+                laid = 0
+            if need_x:
                 dx = torch.empty(T, K, dtype=dtype, device=dev)
-                _lib.check(lib.nnue_grouped_linear_bwd_input(_ptr(dyr), lddy, _ptr(w), ldw, _ptr(plan), _ptr(dx), T, K, N, E,
+                _lib.check(lib.nnue_grouped_linear_bwd_input(_ptr(dyr), lddy, laid, _ptr(w), ldw, _ptr(plan), _ptr(dx), T, K, N, E,
                                                              TYPES[dtype], s), "nnue_grouped_linear_bwd_input")
-            need_b = ctx.needs_input_grad[2] and ctx.b_like is not None
-            if ctx.needs_input_grad[1] or need_b:
+            if need_b:
+                db = torch.empty(ctx.b_like[1], dtype=ctx.b_like[0], device=dev)
+            if need_w:
                 w_dtype, w_shape = ctx.w_like
-                dw = torch.empty(E * N, K, dtype=w_dtype, device=dev)
-                if need_b:
-                    db = torch.empty(ctx.b_like[1], dtype=ctx.b_like[0], device=dev)
+                dw = torch.empty(w_shape, dtype=w_dtype, device=dev)
                 _lib.check(lib.nnue_grouped_linear_bwd_weight(
-                    _ptr(dyr), lddy, _ptr(x), ldx, _ptr(plan), _ptr(dw), TYPES[w_dtype], _ptr(db),
+                    _ptr(dyr), _ptr(part), _ptr(x), _ptr(plan), _ptr(dw), TYPES[w_dtype], _ptr(db),
                     0 if db is None else TYPES[db.dtype], T, K, N, E, TYPES[dtype], s), "nnue_grouped_linear_bwd_weight")
-                dw = dw.view(w_shape) if ctx.needs_input_grad[1] else None
+            elif need_b:
+                _lib.check(lib.nnue_group_sums(_ptr(part), _ptr(plan), _ptr(db), TYPES[db.dtype], T, N, E, s), "nnue_group_sums")
         return dx, dw, db, None, None
 
 
@@ -166,7 +194,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
                    out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y[p] = weight[b(p)] x[p] + bias[b(p)], zeros for rows of no bucket.
 
-    x       bf16 or fp16 [T, K], any strides (rows that do not start at multiples of 16 bytes are copied first)
+    x       bf16 or fp16 [T, K], any strides
     weight  [count * N, K] or [count, N, K], of x's type or fp32
     bias    count * N numbers of x's type or fp32, or None
     out_dtype  x's type (default) or float32

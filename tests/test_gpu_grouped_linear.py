@@ -126,6 +126,27 @@ def test_fp32_output_and_no_bias(dev, K, N):
     close(wd.grad.view(-1, K), *ref["dw"], "dw")
 
 
+def test_each_gradient_alone(dev):
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator().manual_seed(13)
+    for T in (20, 700):  # few rows per bucket, and many
+        count, K, N = 4, 96, 72
+        b = _ids(T, count, T, padding=True)
+        x = torch.randn(T, K, generator=g).half()
+        w, bias = torch.randn(count * N, K, generator=g).half(), torch.randn(count * N, generator=g).half()
+        dy = torch.randn(T, N, generator=g).half()
+        ref = linear_ref(x, w, bias, b, count, dy)
+        plan = GroupPlan(b.to(dev), count)
+        for i, name in enumerate(("dx", "dw", "db")):
+            ts = [t.to(dev).requires_grad_(i == j) for j, t in enumerate((x, w, bias))]
+            y = grouped_linear(*ts, plan)
+            y.backward(dy.to(dev))
+            close(y, *ref["y"], "y")
+            close(ts[i].grad, *ref[name], name)
+            assert all(t.grad is None for j, t in enumerate(ts) if j != i)
+
+
 def test_strides_and_alignments(dev):
     """Column slices at every offset, transposed and expanded operands."""
     from nnue_pytorch_b200 import GroupPlan, grouped_linear

@@ -34,8 +34,8 @@ def test_grouped_linear_arguments(lib):
     BF16, F16, F32, E4M3 = 1, 2, 0, 3
     P = 1 << 20  # an aligned address that no refused call reads
 
-    def fwd(x=P, ldx=64, w=P, ldw=64, bias=None, bt=0, plan=P, y=P, yt=BF16, T=8, K=64, N=16, E=2, type=BF16):
-        return lib.nnue_grouped_linear_fwd(x, ldx, w, ldw, bias, bt, plan, y, yt, T, K, N, E, type, None)
+    def fwd(x=P, ldx=64, laid=0, w=P, ldw=64, bias=None, bt=0, plan=P, y=P, yt=BF16, T=8, K=64, N=16, E=2, type=BF16):
+        return lib.nnue_grouped_linear_fwd(x, ldx, laid, w, ldw, bias, bt, plan, y, yt, T, K, N, E, type, None)
 
     assert fwd(T=0) == 0  # an empty batch needs no device
     assert fwd(T=-1) == -1 and fwd(K=0) == -1 and fwd(N=0) == -1 and fwd(E=0) == -1
@@ -46,15 +46,22 @@ def test_grouped_linear_arguments(lib):
     assert fwd(ldx=66) == -2 and fwd(x=P + 2) == -2 and fwd(ldw=68) == -2 and fwd(y=P + 4) == -2
     assert "16 bytes" in _message(lib) or "unaligned" in _message(lib)
 
-    def dx(dy=P, lddy=16, w=P, ldw=64, plan=P, out=P, T=8, K=64, N=16, E=2, type=F16):
-        return lib.nnue_grouped_linear_bwd_input(dy, lddy, w, ldw, plan, out, T, K, N, E, type, None)
+    def dx(dy=P, lddy=16, laid=0, w=P, ldw=64, plan=P, out=P, T=8, K=64, N=16, E=2, type=F16):
+        return lib.nnue_grouped_linear_bwd_input(dy, lddy, laid, w, ldw, plan, out, T, K, N, E, type, None)
 
     assert dx(T=0) == 0 and dx(dy=None) == -1 and dx(lddy=17) == -2 and dx(lddy=15) == -1 and dx(out=None) == -2 and dx(type=7) == -4
 
-    def dw(dy=P, lddy=16, x=P, ldx=64, plan=P, out=P, ot=F32, db=None, bt=0, T=8, K=64, N=16, E=2, type=F16):
-        return lib.nnue_grouped_linear_bwd_weight(dy, lddy, x, ldx, plan, out, ot, db, bt, T, K, N, E, type, None)
+    def dw(dy=P, sums=P, x=P, plan=P, out=P, ot=F32, db=None, bt=0, T=8, K=64, N=16, E=2, type=F16):
+        return lib.nnue_grouped_linear_bwd_weight(dy, sums, x, plan, out, ot, db, bt, T, K, N, E, type, None)
 
-    assert dw(ot=BF16) == -4 and dw(db=P, bt=E4M3) == -4 and dw(x=None) == -1 and dw(ldx=60) == -1 and dw(out=None) == -2
+    assert dw(ot=BF16) == -4 and dw(db=P, bt=E4M3) == -4 and dw(x=None) == -1 and dw(dy=P + 2) == -2 and dw(out=None) == -2
+    assert dw(db=P, sums=None) == -1 and "sums" in _message(lib)
+    rows = lambda **k: lib.nnue_group_rows(*({**dict(s=P, st=F32, ld=64, plan=P, d=P, t=BF16, sums=None, T=4, c=64, E=2), **k}.values()), None)  # noqa: E731
+    assert rows(T=0) == 0 and rows(T=-1) == -1 and rows(ld=63) == -1 and rows(c=0) == -1 and rows(E=0) == -1 and rows(E=1025) == -4
+    assert rows(st=E4M3) == -4 and rows(t=F32) == -4 and rows(s=None) == -1 and rows(d=P + 8) == -2 and rows(plan=P + 4) == -2
+    assert lib.nnue_group_rows_bytes(100, 20, 8) >= 100 * 24 * 2 and lib.nnue_group_rows_bytes(-1, 20, 8) == 0
+    assert lib.nnue_group_sums_bytes(300, 20, 8) >= 4 * 20 * 4 and lib.nnue_group_sums_bytes(300, 0, 8) == 0
+    assert lib.nnue_group_sums(None, P, P, F32, 4, 8, 2, None) == -1 and lib.nnue_group_sums(P, P, P, E4M3, 4, 8, 2, None) == -4
     assert lib.nnue_pack_rows(P, F32, 4, P, E4M3, 4, 1, 4, None) == -4
     assert lib.nnue_pack_rows(P, F32, 3, P, BF16, 4, 1, 4, None) == -1
     assert lib.nnue_pack_rows(None, F32, 4, None, BF16, 8, 1, 4, None) == -1
