@@ -797,12 +797,16 @@ int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_sums,
  * Numbers that are not finite become NaN in E4M3 and stay what they are in E5M2.
  * rows:  x [T, K] (F32, BF16 or F16, pitch ldx) -> q [T, K] (pitch ldq, at most
  *        the row length rounded up to 128; columns [K, ldq) become zero),
- *        scale [T, ceil(K / 128)]
+ *        scale [T, ceil(K / 128)].  With a plan (of T rows and E buckets) q's rows
+ *        are laid out by bucket as nnue_group_rows lays them, at a pitch of K rounded
+ *        up to 16 (ldq is not looked at), and what lies between buckets is left as it
+ *        is; scale stays in the batch's order, and rows without a bucket get none.
  * tiles: w [E, N, K] (pitch ldw) -> q [E, N, K], scale [E, ceil(N / 128),
  *        ceil(K / 128)]; tiles start anew in every bucket. */
 int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, void* q,
                            int64_t ldq, float* scale, int64_t T, int64_t K,
-                           int32_t format, void* stream);
+                           int32_t format, const void* plan, int32_t E,
+                           void* stream);
 int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
                             int64_t ldq, float* scale, int32_t E, int64_t N,
                             int64_t K, int32_t format, void* stream);
@@ -812,8 +816,11 @@ int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
  * x [T, K] and w [E, N, K] of one 8-bit format, pitches that are multiples of 16,
  * scales as the quantisers lay them out (any fp32 values, not only powers of
  * two), bias [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are
- * fp32.  plan NULL: E = 1 and every row belongs to the one matrix. */
-int nnue_fp8_linear_fwd(const void* x, int64_t ldx, const float* x_scale,
+ * fp32.  plan NULL: E = 1 and every row belongs to the one matrix.  With a plan, x
+ * is laid out by bucket (`laid`; ldx is not looked at) or in the batch's order,
+ * which suits a few rows per bucket. */
+int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid,
+                        const float* x_scale,
                         const void* w, int64_t ldw, const float* w_scale,
                         const float* bias, const void* plan, void* y,
                         int32_t y_type, int64_t T, int64_t K, int64_t N,

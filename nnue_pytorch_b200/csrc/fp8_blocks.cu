@@ -48,59 +48,162 @@ __device__ __forceinline__ uint8_t to_fp8(float v, int format) {
     return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, format == NNUE_T_E4M3 ? __NV_E4M3 : __NV_E5M2);
 }
 
-// One warp per row block.  q's columns [K, ldq) become zero.
-__global__ void __launch_bounds__(kThreads)
-    k_fp8_rows(const void* __restrict__ x, int type, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
-               int64_t T, int64_t K, int format) {
-    const int64_t C = (K + kFp8Block - 1) / kFp8Block;
-    const int lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
-    if (i >= T * C) return;
-    const int64_t t = i / C, c = i % C;
-    float v[4];
-    uint32_t most = 0;
+constexpr int kLaneNumbers = 16;                                 // consecutive numbers of a lane: 16 bytes of q
+constexpr int kWarpNumbers = 32 * kLaneNumbers;                  // four blocks of a row
+constexpr int kBlockLanes = kFp8Block / kLaneNumbers;            // 8
+
+// v[i] = p[at + i], zeros from i = left on
+__device__ __forceinline__ void load_sixteen(const void* p, int type, int64_t at, int left, bool vec, float (&v)[kLaneNumbers]) {
+    if (vec && left >= kLaneNumbers) {
+        if (type == NNUE_T_F32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t k = c * kFp8Block + j * 32 + lane;
-        v[j] = k < K ? load_as_float(x, type, t * ldx + k) : 0.f;
-        most = max(most, finite_abs_bits(v[j]));
-    }
-    most = __reduce_max_sync(kFullMask, most);
-    const int e = fp8_scale_exponent(most, format);
-    const float inverse = power_of_two(-e);
+            for (int i = 0; i < 4; ++i) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at) + i);
+                v[4 * i] = f.x;
+                v[4 * i + 1] = f.y;
+                v[4 * i + 2] = f.z;
+                v[4 * i + 3] = f.w;
+            }
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t k = c * kFp8Block + j * 32 + lane;
-        if (k < ldq) q[t * ldq + k] = to_fp8(v[j] * inverse, format);
+            for (int i = 0; i < 2; ++i) {
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at) + i);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (type == NNUE_T_BF16) {
+                        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+                        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    } else {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                        v[8 * i + 2 * j] = f.x;
+                        v[8 * i + 2 * j + 1] = f.y;
+                    }
+                }
+            }
+        }
+        return;
     }
-    if (lane == 0) scale[i] = power_of_two(e);
+#pragma unroll
+    for (int i = 0; i < kLaneNumbers; ++i) v[i] = i < left ? load_as_float(p, type, at + i) : 0.f;
 }
 
-// One CTA per 128 x 128 tile.
-__global__ void __launch_bounds__(kThreads)
+// bits of the largest finite |v|
+__device__ __forceinline__ uint32_t largest_bits(const float (&v)[kLaneNumbers]) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < kLaneNumbers; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
+    if (most < 0x7f800000u) return most;
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < kLaneNumbers; ++i) most = max(most, finite_abs_bits(v[i]));
+    return most;
+}
+
+// q[at + i] = v[i] * inverse in 8 bits, `room` of them
+__device__ __forceinline__ void store_sixteen(uint8_t* q, int64_t at, int room, bool vec, const float (&v)[kLaneNumbers], float inverse,
+                                              int format) {
+    uint32_t raw = 0;
+#pragma unroll
+    for (int i = 0; i < kLaneNumbers; ++i) raw = max(raw, __float_as_uint(v[i]) & 0x7fffffffu);
+    uint32_t w[4];
+    if (raw < 0x7f800000u) {
+        const __nv_fp8_interpretation_t kind = format == NNUE_T_E4M3 ? __NV_E4M3 : __NV_E5M2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inverse, v[4 * i + 1] * inverse), __NV_SATFINITE, kind);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inverse, v[4 * i + 3] * inverse), __NV_SATFINITE, kind);
+            w[i] = lo | hi << 16;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[i] |= (uint32_t)to_fp8(v[4 * i + j] * inverse, format) << (8 * j);
+        }
+    }
+    if (vec && room >= kLaneNumbers) {
+        *reinterpret_cast<uint4*>(q + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kLaneNumbers; ++i)
+            if (i < room) q[at + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+}
+
+struct Fp8Args {
+    GroupPlanView plan;
+    const void* x;
+    uint8_t* q;
+    float* scale;
+    int64_t ldx, ldq, T;
+    int32_t K, type, format, E;
+    int32_t warps;        // per row: four blocks each
+    int32_t vec_x, vec_q;
+};
+
+// A warp quantises four blocks of a row: a lane holds 16 consecutive numbers (one 16-byte store), eight lanes a block.
+// Bound by HBM; 32 (64) bytes per lane in flight.  Laid out by bucket: the rows are walked by the plan's tiles.
+template <bool LAID>
+__global__ void __launch_bounds__(kThreads) k_fp8_rows(const __grid_constant__ Fp8Args a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t i = (int64_t)blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
+    const int64_t r = i / a.warps;
+    const int part = (int)(i - r * a.warps);
+    int64_t from = r, to = r;
+    if (LAID) {
+        const int64_t t = r / kGroupRows;
+        if (t >= __ldg(a.plan.n_tiles)) return;
+        const int4 tile = __ldg(reinterpret_cast<const int4*>(a.plan.tiles) + t);
+        const int in = (int)(r - t * kGroupRows);
+        if (tile.x >= a.E || in >= tile.z) return;
+        from = __ldg(a.plan.order + tile.y + in);
+        to = tile.w + in;
+    } else if (r >= a.T) {
+        return;
+    }
+    const int k = part * kWarpNumbers + lane * kLaneNumbers, C = (a.K + kFp8Block - 1) / kFp8Block;
+    float v[kLaneNumbers];
+    load_sixteen(a.x, a.type, from * a.ldx + k, a.K - k, a.vec_x, v);
+    uint32_t most = largest_bits(v);
+#pragma unroll
+    for (int d = 1; d < kBlockLanes; d <<= 1) most = max(most, __shfl_xor_sync(kFullMask, most, d));
+    const int e = fp8_scale_exponent(most, a.format);
+    store_sixteen(a.q, to * a.ldq + k, (int)min((int64_t)kLaneNumbers, a.ldq - k), a.vec_q, v, power_of_two(-e), a.format);
+    const int c = k / kFp8Block;
+    if (lane % kBlockLanes == 0 && c < C) a.scale[from * C + c] = power_of_two(e);
+}
+
+// One CTA per 128 x 128 tile: every number is read once and held in registers, 64 per thread, until the scale is known.
+__global__ void __launch_bounds__(kThreads, 2)
     k_fp8_tiles(const void* __restrict__ w, int type, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
-                int64_t N, int64_t K, int format) {
+                int64_t N, int64_t K, int format, int vec_w, int vec_q) {
     const int64_t C = (K + kFp8Block - 1) / kFp8Block, R = (N + kFp8Block - 1) / kFp8Block;
     const int64_t tile = blockIdx.x, c = tile % C, r = tile / C % R, e = tile / (C * R);
-    const int col = threadIdx.x & 127, sub = threadIdx.x >> 7;
-    const int64_t k = c * kFp8Block + col;
-    __shared__ uint32_t s_most;
-    if (threadIdx.x == 0) s_most = 0;
-    __syncthreads();
+    const int64_t k = c * kFp8Block + (threadIdx.x % kBlockLanes) * kLaneNumbers;
+    const int64_t n0 = r * kFp8Block + threadIdx.x / kBlockLanes;
+    constexpr int kRows = kThreads / kBlockLanes;  // 32 rows at once
+    float v[4][kLaneNumbers];
     uint32_t most = 0;
-    for (int j = sub; j < kFp8Block; j += 2) {
-        const int64_t n = r * kFp8Block + j;
-        if (n < N && k < K) most = max(most, finite_abs_bits(load_as_float(w, type, (e * N + n) * ldw + k)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + j * kRows;
+        load_sixteen(w, type, (e * N + n) * ldw + k, n < N ? (int)(K - k) : 0, vec_w, v[j]);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = max(most, largest_bits(v[j]));
+    __shared__ uint32_t s_most[kWarpsPerCta];
     most = __reduce_max_sync(kFullMask, most);
-    if ((threadIdx.x & 31) == 0) atomicMax(&s_most, most);
+    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
     __syncthreads();
-    const int x = fp8_scale_exponent(s_most, format);
-    const float inverse = power_of_two(-x);
-    for (int j = sub; j < kFp8Block; j += 2) {
-        const int64_t n = r * kFp8Block + j;
-        if (n < N && k < ldq)
-            q[(e * N + n) * ldq + k] = k < K ? to_fp8(load_as_float(w, type, (e * N + n) * ldw + k) * inverse, format) : 0;
+#pragma unroll
+    for (int j = 0; j < kWarpsPerCta; ++j) most = max(most, s_most[j]);
+    const int x = fp8_scale_exponent(most, format);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t n = n0 + j * kRows;
+        if (n < N) store_sixteen(q, (e * N + n) * ldq + k, (int)min((int64_t)kLaneNumbers, ldq - k), vec_q, v[j], power_of_two(-x), format);
     }
     if (threadIdx.x == 0) scale[tile] = power_of_two(x);
 }
@@ -120,14 +223,37 @@ static int check_fp8(const char* what, const void* x, int32_t type, int64_t ldx,
 }
 
 extern "C" int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t T,
-                                      int64_t K, int32_t format, void* stream) {
-    if (int st = check_fp8("nnue_fp8_quantize_rows", x, type, ldx, q, ldq, scale, T, K, format)) return st;
+                                      int64_t K, int32_t format, const void* plan, int32_t E, void* stream) {
+    const char* what = "nnue_fp8_quantize_rows";
+    if (plan) {
+        NNUE_REQUIRE(E > 0 && E <= kMaxGroups && T <= NNUE_GROUP_MAX_ROWS && aligned16(plan), NNUE_ERR_ARG, "%s: bad plan", what);
+        ldq = (K + 15) / 16 * 16;
+    }
+    if (int st = check_fp8(what, x, type, ldx, q, ldq, scale, T, K, format)) return st;
+    NNUE_REQUIRE(K < (1 << 24), NNUE_ERR_UNSUPPORTED, "%s: rows of %lld numbers", what, (long long)K);
     if (T == 0) return NNUE_OK;
-    const int64_t blocks = (T * ((K + kFp8Block - 1) / kFp8Block) + kWarpsPerCta - 1) / kWarpsPerCta;
-    NNUE_REQUIRE(blocks <= 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "nnue_fp8_quantize_rows: too many blocks");
+    Fp8Args a = {};
+    if (plan) a.plan = group_view(plan, T, E);
+    a.x = x;
+    a.q = static_cast<uint8_t*>(q);
+    a.scale = scale;
+    a.ldx = ldx;
+    a.ldq = ldq;
+    a.T = T;
+    a.K = (int32_t)K;
+    a.type = type;
+    a.format = format;
+    a.E = E;
+    a.warps = (int32_t)((K + kWarpNumbers - 1) / kWarpNumbers);
+    a.vec_x = aligned16(x) && ldx * type_bytes(type) % 16 == 0;
+    a.vec_q = aligned16(q) && ldq % 16 == 0;
+    const int64_t rows = plan ? group_max_tiles(T, E) * kGroupRows : T;
+    const int64_t blocks = (rows * a.warps + kWarpsPerCta - 1) / kWarpsPerCta;
+    NNUE_REQUIRE(blocks <= 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "%s: too many blocks", what);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("fp8_rows", s);
-    k_fp8_rows<<<(unsigned)blocks, kThreads, 0, s>>>(x, type, ldx, static_cast<uint8_t*>(q), ldq, scale, T, K, format);
+    if (plan) k_fp8_rows<true><<<(unsigned)blocks, kThreads, 0, s>>>(a);
+    else k_fp8_rows<false><<<(unsigned)blocks, kThreads, 0, s>>>(a);
     note_launches(1);
     NNUE_CUDA_TRY(cudaGetLastError());
     return NNUE_OK;
@@ -142,7 +268,8 @@ extern "C" int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw,
     NNUE_REQUIRE(tiles <= 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "nnue_fp8_quantize_tiles: too many tiles");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("fp8_tiles", s);
-    k_fp8_tiles<<<(unsigned)tiles, kThreads, 0, s>>>(w, type, ldw, static_cast<uint8_t*>(q), ldq, scale, N, K, format);
+    k_fp8_tiles<<<(unsigned)tiles, kThreads, 0, s>>>(w, type, ldw, static_cast<uint8_t*>(q), ldq, scale, N, K, format,
+                                                     aligned16(w) && ldw * type_bytes(type) % 16 == 0, aligned16(q) && ldq % 16 == 0);
     note_launches(1);
     NNUE_CUDA_TRY(cudaGetLastError());
     return NNUE_OK;

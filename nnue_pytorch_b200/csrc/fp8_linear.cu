@@ -1,60 +1,365 @@
-// Linear layer on 8-bit operands with a scale per 128 inputs of a row and per 128 x 128 tile of the weights:
+// Linear layer on 8-bit operands with a scale per 128 inputs of a row and per 128 x 128 tile of the weights, dense or
+// bucketed, on the 5th-generation tensor cores:
 //   y[p, n] = sum_c sx[p, c] sw[b, n / 128, c] sum_{k in block c} x[p, k] w[b, n, k] + bias[b, n]
-// First form: one thread per output element, fp32 sums.
-#include "grouped.cuh"
-
-#include <cuda_fp8.h>
+//
+// A stage is one block of 128 inputs (a 128-byte swizzle row per operand row), four tcgen05.mma of 32 inputs each, whose
+// sum goes to an accumulator of its own in tensor memory; eight warps take the accumulators one after the other, multiply
+// them by sx * sw and add them up in fp32 registers (a thread holds half a row of the tile: its row's scale is one number,
+// and so is the weights' on its columns).  The scales may be any fp32 numbers.  The tensor core takes 512 cycles for a
+// stage of 128 x 256, reading the accumulator 256, the multiply-adds 256 issue slots of each quarter: they overlap, two
+// accumulators (four of 128 columns) being in turn.
+// Copies, pairs of SMs, split sums and bounded waits as in the 16-bit kernel (grouped_linear.cu).  Rows come laid out by
+// bucket (the quantiser leaves them so), in their own order where there is one matrix, or are gathered by TMA, four per
+// copy, where a bucket has few.
+#include "grouped_tc.cuh"
 
 namespace nnue {
 
-constexpr int kF = 32;
-constexpr int kFp8Block = 128;
+constexpr int kF8K = 128;
+constexpr int kF8ABytes = kGroupRows * 128;
+constexpr int kF8Threads = 320;
 
-__device__ __forceinline__ float from_fp8(uint8_t v, int format) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, format == NNUE_T_E4M3 ? __NV_E4M3 : __NV_E5M2)));
+constexpr int f8_stage_bytes(int bn, int ctas) { return kF8ABytes + bn / ctas * 128; }
+constexpr int f8_stages(int bn, int ctas) { return f8_stage_bytes(bn, ctas) > 32768 ? 4 : f8_stage_bytes(bn, ctas) > 24576 ? 6 : 8; }
+constexpr int f8_accs(int bn) { return bn == 256 ? 2 : 4; }
+constexpr int f8_smem(int bn, int ctas) { return 1024 + f8_stages(bn, ctas) * f8_stage_bytes(bn, ctas) + 8 * kStagingBytes + 256; }
+
+struct F8Args {
+    GroupPlanView plan;
+    RowsOut o;
+    const float *x_scale, *w_scale, *bias;
+    int32_t T, E, N, K;
+    int32_t C, R;        // blocks along K and along N
+    int32_t col_tiles;
+    int32_t dense;       // one matrix, rows in their own order
+    int32_t gather;
+    uint32_t idesc;
+    unsigned long long* status;
+};
+
+struct F8Tile {
+    int32_t bucket, first, count, place, col0, c0, c1;
+    bool live;
+};
+
+template <int BN, int CTAS, bool SPLIT>
+__device__ __forceinline__ F8Tile f8_tile(const F8Args& a, int t, int rank, int ranks) {
+    F8Tile x;
+    const int rt = t / a.col_tiles;
+    x.col0 = (t - rt * a.col_tiles) * BN;
+    if (a.dense) {
+        x.bucket = 0;
+        x.first = x.place = rt * (kGroupRows * CTAS);
+        x.count = min(kGroupRows * CTAS, a.T - x.first);
+    } else {
+        const int4 g = __ldg(reinterpret_cast<const int4*>(CTAS == 2 ? a.plan.pairs : a.plan.tiles) + rt);
+        x.bucket = g.x;
+        x.first = g.y;
+        x.count = g.z;
+        x.place = g.w;
+    }
+    x.live = x.bucket < a.E;
+    const int chunks = x.live ? a.C : 0;
+    x.c0 = SPLIT ? chunks * rank / ranks : 0;
+    x.c1 = SPLIT ? chunks * (rank + 1) / ranks : chunks;
+    return x;
 }
 
-__global__ void __launch_bounds__(kF* kF)
-    k_fp8_linear(const uint8_t* x, int64_t ldx, const float* sx, const uint8_t* w, int64_t ldw, const float* sw, const float* bias,
-                 const int32_t* plan, void* y, int y_type, int64_t T, int64_t K, int64_t N, int E, int format) {
-    const int64_t t = blockIdx.y / (kGroupRows / kF);
-    GroupTile tile{0, (int32_t)(t * kGroupRows), (int32_t)min((int64_t)kGroupRows, T - t * kGroupRows), 0};
-    const GroupPlanView view = group_view(plan, T, E);
-    if (plan) {
-        if (t >= *view.n_tiles) return;
-        tile = view.tiles[t];
-    }
-    __shared__ float sa[kF][kF + 1], sb[kF][kF + 1];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int row = blockIdx.y % (kGroupRows / kF) * kF + ty;
-    const int64_t p = row < tile.count ? (plan ? view.order[tile.start + row] : tile.start + row) : -1;
-    const int64_t C = (K + kFp8Block - 1) / kFp8Block, R = (N + kFp8Block - 1) / kFp8Block;
-    for (int64_t n0 = (int64_t)blockIdx.x * kF; n0 < N; n0 += (int64_t)gridDim.x * kF) {
-        float acc = 0.f;
-        if (tile.bucket < E) {
-            const int64_t wrow = (int64_t)tile.bucket * N;
-            for (int64_t c = 0; c < C; ++c) {
-                float part = 0.f;
-                for (int64_t k0 = c * kFp8Block; k0 < min(K, (c + 1) * kFp8Block); k0 += kF) {
-                    sa[ty][tx] = p >= 0 && k0 + tx < K ? from_fp8(x[p * ldx + k0 + tx], format) : 0.f;
-                    sb[tx][ty] = n0 + ty < N && k0 + tx < K ? from_fp8(w[(wrow + n0 + ty) * ldw + k0 + tx], format) : 0.f;
-                    __syncthreads();
-                    for (int i = 0; i < kF; ++i) part = fmaf(sa[ty][i], sb[i][tx], part);
-                    __syncthreads();
-                }
-                if (p >= 0) acc = fmaf(part, sx[p * C + c] * sw[((int64_t)tile.bucket * R + n0 / kFp8Block) * C + c], acc);
-            }
-            if (bias && n0 + tx < N) acc += bias[wrow + n0 + tx];
+template <int BN, int CTAS, bool SPLIT>
+__device__ __forceinline__ bool f8_copy_role(const F8Args& a, const CUtensorMap* map_x, const CUtensorMap* map_w, uint32_t ring,
+                                             uint64_t* full, uint64_t* empty, int t0, int stride, int tiles, int rank, int ranks) {
+    constexpr bool PAIR = CTAS == 2;
+    const int lane = threadIdx.x & 31, side = PAIR ? rank : 0;
+    StageRing<f8_stages(BN, CTAS)> at;
+    bool ok = true;
+    for (int t = t0; t < tiles && ok; t += stride) {
+        const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t, rank, ranks);
+        if (x.c0 == x.c1) continue;
+        const bool gather = !PAIR && a.gather;
+        // the bytes that complete a stage: both CTAs' of a pair, announced by the first
+        const int bytes = BN * 128 + (gather ? ((x.count + 3) >> 2) * 512 : (PAIR && x.count > kGroupRows ? 2 : 1) * kF8ABytes);
+        int rows[4];
+        if (gather) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rows[j] = 4 * lane + j < x.count ? __ldg(a.plan.order + x.first + 4 * lane + j) : a.T;
         }
-        if (p >= 0 && n0 + tx < N) store_from_float(y, y_type, p * N + n0 + tx, acc);
+        for (int c = x.c0; c < x.c1; ++c) {
+            if (lane == 0) ok = mbar_wait_timed(empty + at.stage, at.phase ^ 1u);
+            ok = __shfl_sync(kFullMask, (int)ok, 0) != 0;
+            if (!ok) break;
+            const uint32_t sa = ring + at.stage * f8_stage_bytes(BN, CTAS), sb = sa + kF8ABytes;
+            const uint32_t bar = PAIR ? map_rank(full + at.stage, 0) : smem_u32(full + at.stage);
+            if (lane == 0) {
+                if (!PAIR || rank == 0) mbar_expect_tx(full + at.stage, bytes);
+                if (!gather && x.count > side * kGroupRows) tma_tile_2d<PAIR>(sa, map_x, c * kF8K, x.place + side * kGroupRows, bar);
+                tma_tile_3d<PAIR>(sb, map_w, c * kF8K, x.col0 + side * (BN / CTAS), x.bucket, bar);
+            }
+            if (gather) {
+                __syncwarp();
+                if (4 * lane < x.count) tma_gather4(sa + lane * 512, map_x, c * kF8K, rows[0], rows[1], rows[2], rows[3], bar);
+            }
+            at.next();
+        }
     }
+    return ok;
+}
+
+template <int BN, int CTAS, bool SPLIT>
+__device__ __forceinline__ bool f8_issue_role(const F8Args& a, uint32_t tmem, uint32_t ring, uint64_t* full, uint64_t* empty,
+                                              uint64_t* done, uint64_t* taken, uint64_t* drained, int t0, int stride, int tiles,
+                                              int rank, int ranks) {
+    constexpr bool PAIR = CTAS == 2;
+    StageRing<f8_stages(BN, CTAS)> at;
+    StageRing<f8_accs(BN)> acc;
+    bool ok = true;
+    for (int t = t0; t < tiles && ok; t += stride) {
+        const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t, rank, ranks);
+        for (int c = x.c0; c < x.c1; ++c) {
+            ok = mbar_wait_timed(taken + acc.stage, acc.phase ^ 1u) && mbar_wait_timed(full + at.stage, at.phase);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sa = ring + at.stage * f8_stage_bytes(BN, CTAS);
+            const uint64_t da = umma_desc_sw128(sa, 16), db = umma_desc_sw128(sa + kF8ABytes, 16);
+            const int steps = min(4, (a.K - c * kF8K + 31) >> 5);  // instructions of 32 inputs
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < steps) umma_f8<PAIR>(tmem + acc.stage * BN, da + 2 * k, db + 2 * k, a.idesc, k != 0);
+            umma_commit_to<PAIR>(empty + at.stage);
+            umma_commit_to<PAIR>(done + acc.stage);
+            at.next();
+            acc.next();
+        }
+    }
+    if (!ok) {  // instructions in flight finish before the tensor memory is freed
+        umma_commit_to<PAIR>(drained);
+        mbar_wait_timed(drained, 0);
+    }
+    return ok;
+}
+
+// s * v + acc, two numbers at once, each product-sum rounded once
+__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t v1, float s) {
+    unsigned long long a, v, ss;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(ss) : "f"(s));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(v), "l"(ss));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
+}
+
+template <int BN, int CTAS, bool SPLIT>
+__global__ void __launch_bounds__(kF8Threads, 1)
+    k_fp8_linear(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ F8Args a) {
+    constexpr bool PAIR = CTAS == 2;
+    constexpr int S = f8_stages(BN, CTAS), A = f8_accs(BN), HALF = BN / 2;  // HALF: columns of an output warp
+    constexpr uint32_t kTmemCols = A * BN;
+    constexpr int kPartPitch = BN + 4;  // floats per row of a partial tile
+    static_assert(!(PAIR && SPLIT), "no such variant");
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
+    unsigned char* staging = ring_ptr + S * f8_stage_bytes(BN, CTAS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * kStagingBytes);  // [S] a stage's copies are in (pair: the first CTA's)
+    uint64_t* empty = full + S;                                                 // [S] a stage may be overwritten
+    uint64_t* done = empty + S;                                                 // [A] an accumulator is complete
+    uint64_t* taken = done + A;                                                 // [A] an accumulator has been read
+    uint64_t* drained = taken + A;                                              // [1]
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int rank = 0, ranks = 1;
+    if (SPLIT || PAIR) {
+        rank = (int)cluster_rank();
+        uint32_t n;
+        asm volatile("mov.u32 %0, %cluster_nctaid.x;" : "=r"(n));
+        ranks = (int)n;
+    }
+    const int row_tiles = a.dense ? (a.T + kGroupRows * CTAS - 1) / (kGroupRows * CTAS) : __ldg(a.plan.n_tiles + (PAIR ? 1 : 0));
+    const int tiles = row_tiles * a.col_tiles;
+    const int t0 = (int)blockIdx.x / ranks, stride = (int)gridDim.x / ranks;  // split: at most one tile per cluster
+    if (t0 >= tiles) return;                                                  // (the whole cluster)
+
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, 1);
+        }
+        for (int s = 0; s < A; ++s) {
+            mbar_init(done + s, 1);
+            mbar_init(taken + s, 8 * CTAS);
+        }
+        mbar_init(drained, 1);
+        fence_barrier_init();
+        prefetch_map(&map_x);
+        prefetch_map(&map_w);
+    }
+    if (warp == 1) tmem_alloc<PAIR>(s_tmem, kTmemCols);
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();  // the other CTA's barriers are there
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+
+    bool ok = true;
+    if (warp == 0) {
+        ok = f8_copy_role<BN, CTAS, SPLIT>(a, &map_x, &map_w, ring, full, empty, t0, stride, tiles, rank, ranks);
+    } else if (warp == 1) {
+        if (lane == 0 && !(PAIR && rank != 0))
+            ok = f8_issue_role<BN, CTAS, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2;  // the quarter of tensor memory's lanes, the half of the columns
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + half * HALF;
+        unsigned char* stg = staging + (warp - 2) * kStagingBytes;
+        StageRing<A> at;
+        for (int t = t0; t < tiles && ok; t += stride) {
+            const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t, rank, ranks);
+            const int r = (PAIR ? rank * kGroupRows : 0) + q * 32 + lane;
+            const int32_t my_row = r >= x.count ? -1 : a.dense ? x.first + r : __ldg(a.plan.order + x.first + r);
+            const int col = x.col0 + half * HALF;
+            const float* sx = a.x_scale + (int64_t)max(my_row, 0) * a.C;
+            const float* sw = a.w_scale + ((int64_t)(x.live ? x.bucket : 0) * a.R + min(col / kF8K, a.R - 1)) * a.C;
+            float acc[HALF];
+#pragma unroll
+            for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
+            float s_next = x.c1 > x.c0 && my_row >= 0 ? __ldg(sx + x.c0) * __ldg(sw + x.c0) : 0.f;
+            for (int c = x.c0; c < x.c1; ++c) {
+                const float s = s_next;
+                if (c + 1 < x.c1 && my_row >= 0) s_next = __ldg(sx + c + 1) * __ldg(sw + c + 1);
+                ok = mbar_wait_warp(done + at.stage, at.phase);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int h = 0; h < HALF; h += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(from + at.stage * BN + h, v);
+                    tmem_wait_ld();
+                    if (h + 32 == HALF) {  // the accumulator goes back before the last products
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR) mbar_arrive_cluster(map_rank(taken + at.stage, 0));
+                            else mbar_arrive(taken + at.stage);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) fma2(acc[h + j], acc[h + j + 1], v[j], v[j + 1], s);
+                }
+                at.next();
+            }
+            if (!ok) break;
+            if (SPLIT) {
+                // the last accumulator is complete, so nothing reads the ring any more: it takes the partial tile
+                float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * kPartPitch + half * HALF;
+#pragma unroll
+                for (int j = 0; j < HALF; j += 4) *reinterpret_cast<float4*>(part + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                break;
+            }
+            if (!__any_sync(kFullMask, my_row >= 0) || col >= a.o.cols) continue;
+            if (a.bias && x.live) {
+                const float* b = a.bias + (int64_t)x.bucket * a.N + col;
+#pragma unroll
+                for (int j = 0; j < HALF; ++j)
+                    if (col + j < a.o.cols) acc[j] += __ldg(b + j);
+            }
+            if (a.o.type == NNUE_T_F32) {
+#pragma unroll
+                for (int h = 0; h < HALF; h += 32) {
+#pragma unroll
+                    for (int p = 0; p < 8; ++p)
+                        *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+                            make_float4(acc[h + 4 * p], acc[h + 4 * p + 1], acc[h + 4 * p + 2], acc[h + 4 * p + 3]);
+                    copy_rows_out(a.o, stg, 128, my_row, 0, col + h);
+                }
+            } else {
+                constexpr int kPass = HALF < 64 ? HALF : 64;
+#pragma unroll
+                for (int h = 0; h < HALF; h += kPass) {
+#pragma unroll
+                    for (int p = 0; p < kPass / 8; ++p) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[j] = pack_half(acc[h + 8 * p + 2 * j], acc[h + 8 * p + 2 * j + 1], a.o.type);
+                        *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    copy_rows_out(a.o, stg, kPass * 2, my_row, 0, col + h);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (!ok && lane == 0) note_timeout(a.status);
+
+    if (SPLIT) {
+        cluster_sync();
+        // row r of the tile is finished by rank r mod ranks: partial sums in the order of the ranks
+        const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t0, rank, ranks);
+        const int mine = (x.count - rank + ranks - 1) / ranks;
+        for (int i = tid; i < mine * (BN / 4); i += kF8Threads) {
+            const int r = rank + i / (BN / 4) * ranks, c = i % (BN / 4) * 4, col = x.col0 + c;
+            if (col >= a.o.cols) continue;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (x.live) {
+                const uint32_t addr = ring + (uint32_t)(r * kPartPitch + c) * 4;
+                for (int s = 0; s < ranks; ++s) {
+                    const float4 p = ld_cluster4(addr, (uint32_t)s);
+                    v[0] += p.x;
+                    v[1] += p.y;
+                    v[2] += p.z;
+                    v[3] += p.w;
+                }
+                if (a.bias) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < a.o.cols) v[j] += __ldg(a.bias + (int64_t)x.bucket * a.N + col + j);
+                }
+            }
+            const int64_t row = a.dense ? x.first + r : __ldg(a.plan.order + x.first + r), at = row * a.o.ld + col;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < a.o.cols) store_from_float(a.o.out, a.o.type, at + j, v[j]);
+        }
+        cluster_sync();  // nobody leaves while its shared memory is read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync();  // both have read their tensor memory, and nobody's barriers are arrived on any more
+    if (warp == 1) tmem_free<PAIR>(tmem, kTmemCols);
+}
+
+template <int BN, int CTAS, bool SPLIT>
+int f8_launch(const CUtensorMap& mx, const CUtensorMap& mw, const F8Args& a, int64_t tiles, int ranks, cudaStream_t s) {
+    auto kernel = k_fp8_linear<BN, CTAS, SPLIT>;
+    static bool opted[64] = {};  // more than 48 KB of dynamic shared memory needs the opt-in, once per device
+    int dev = 0;
+    NNUE_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !opted[dev]) {
+        NNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, f8_smem(BN, CTAS)));
+        if (dev >= 0 && dev < 64) opted[dev] = true;
+    }
+    const int64_t at_once = sm_count() / CTAS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(SPLIT ? tiles * ranks : (tiles < at_once ? tiles : at_once) * CTAS));
+    cfg.blockDim = dim3(kF8Threads);
+    cfg.dynamicSmemBytes = f8_smem(BN, CTAS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    if (SPLIT || CTAS > 1) {
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)(SPLIT ? ranks : CTAS);
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+    }
+    NNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mx, mw, a));
+    note_launches(1);
+    return NNUE_OK;
 }
 
 }  // namespace nnue
 
 using namespace nnue;
 
-extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, const float* x_scale, const void* w, int64_t ldw,
+extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, const float* x_scale, const void* w, int64_t ldw,
                                    const float* w_scale, const float* bias, const void* plan, void* y, int32_t y_type, int64_t T,
                                    int64_t K, int64_t N, int32_t E, int32_t format, void* stream) {
     const char* what = "nnue_fp8_linear_fwd";
@@ -65,19 +370,52 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, const float* x_sc
     NNUE_REQUIRE(format == NNUE_T_E4M3 || format == NNUE_T_E5M2, NNUE_ERR_UNSUPPORTED, "%s: format %d", what, format);
     NNUE_REQUIRE(is_float_type(y_type), NNUE_ERR_UNSUPPORTED, "%s: output type %d", what, y_type);
     NNUE_REQUIRE(plan || E == 1, NNUE_ERR_ARG, "%s: %d buckets need a plan", what, E);
+    NNUE_REQUIRE(plan || !laid, NNUE_ERR_ARG, "%s: rows laid out by bucket need their plan", what);
     if (T == 0) return NNUE_OK;
     NNUE_REQUIRE(x && w && x_scale && w_scale && y, NNUE_ERR_ARG, "%s: null pointer", what);
+    if (laid) ldx = (K + 15) / 16 * 16;
     NNUE_REQUIRE(ldx >= K && ldw >= K, NNUE_ERR_ARG, "%s: pitch below the row length", what);
     NNUE_REQUIRE(aligned16(x) && aligned16(w) && ldx % 16 == 0 && ldw % 16 == 0, NNUE_ERR_ALIGN,
                  "%s: rows of x and w must start at multiples of 16 bytes", what);
     NNUE_REQUIRE(aligned16(y) && aligned16(plan), NNUE_ERR_ALIGN, "%s: unaligned output or plan", what);
-    const int64_t tiles = plan ? group_max_tiles(T, E) : (T + kGroupRows - 1) / kGroupRows;
-    const dim3 grid((unsigned)((N + kF - 1) / kF), (unsigned)(tiles * (kGroupRows / kF)));
+    F8Args a = {};
+    if (plan) a.plan = group_view(plan, T, E);
+    a.o = rows_out(y, y_type, N);
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.bias = bias;
+    a.T = (int32_t)T;
+    a.E = E;
+    a.N = (int32_t)N;
+    a.K = (int32_t)K;
+    a.C = (int32_t)((K + kF8K - 1) / kF8K);
+    a.R = (int32_t)((N + kF8K - 1) / kF8K);
+    a.dense = !plan;
+    a.gather = plan && !laid;
+    a.status = device_status_ptr();
+    NNUE_REQUIRE(a.status, NNUE_ERR_CUDA, "%s: no device status word", what);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("fp8_linear", s);
-    k_fp8_linear<<<grid, kF * kF, 0, s>>>(static_cast<const uint8_t*>(x), ldx, x_scale, static_cast<const uint8_t*>(w), ldw, w_scale,
-                                          bias, static_cast<const int32_t*>(plan), y, y_type, T, K, N, E, format);
-    note_launches(1);
-    NNUE_CUDA_TRY(cudaGetLastError());
-    return NNUE_OK;
+    const int64_t runs = E < T ? E : T;
+    const TileShape shape = tile_shape(runs, (T + runs - 1) / runs, N, a.C, 64, 256, !a.gather);
+    a.col_tiles = (int32_t)((N + shape.bn - 1) / shape.bn);
+    a.idesc = umma_idesc(format == NNUE_T_E5M2 ? 1u : 0u, (uint32_t)(kGroupRows * shape.ctas), (uint32_t)shape.bn, 0, 0);
+    CUtensorMap mx, mw;
+    {
+        const uint64_t dims[2] = {(uint64_t)K, (uint64_t)(laid ? group_laid_rows(T, E) : T)}, strides[1] = {(uint64_t)ldx};
+        const uint32_t box[2] = {kF8K, a.gather ? 1u : (uint32_t)kGroupRows};
+        if (int st = encode_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, x, dims, strides, box)) return st;
+    }
+    {
+        const uint64_t dims[3] = {(uint64_t)K, (uint64_t)N, (uint64_t)E}, strides[2] = {(uint64_t)ldw, (uint64_t)(N * ldw)};
+        const uint32_t box[3] = {kF8K, (uint32_t)(shape.bn / shape.ctas), 1};
+        if (int st = encode_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w, dims, strides, box)) return st;
+    }
+    const int64_t tiles = (plan ? group_max_tiles(T, E) : (T + kGroupRows - 1) / kGroupRows) * a.col_tiles;
+    NNUE_REQUIRE(tiles * 8 < 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "%s: too many tiles", what);
+    if (shape.ctas == 2) return f8_launch<256, 2, false>(mx, mw, a, tiles, 1, s);
+    const bool split = shape.ranks > 1;
+    if (shape.bn == 64) return split ? f8_launch<64, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<64, 1, false>(mx, mw, a, tiles, 1, s);
+    if (shape.bn == 128) return split ? f8_launch<128, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<128, 1, false>(mx, mw, a, tiles, 1, s);
+    return split ? f8_launch<256, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<256, 1, false>(mx, mw, a, tiles, 1, s);
 }

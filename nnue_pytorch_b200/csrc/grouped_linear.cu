@@ -27,8 +27,7 @@
 //   tensor memory.
 // All orders are fixed by the sizes: results are reproducible.  Every wait is bounded; one that runs out raises the
 // device status word and the CTA leaves, its tensor memory freed; copies in flight are then as old as that wait.
-#include "grouped.cuh"
-#include "tc.cuh"
+#include "grouped_tc.cuh"
 
 namespace nnue {
 
@@ -37,30 +36,27 @@ enum { kModeFwd = 0, kModeDx = 1, kModeDw = 2 };
 constexpr int kGlK = 64;                     // reduction elements per stage: one 128-byte swizzle row
 constexpr int kGlABytes = kGroupRows * 128;  // 16 KiB
 constexpr int kGlBoxBytes = kGlK * 128;      // MN-major block: 64 rows of the reduction x 128 bytes
-constexpr int kGlStageWarp = 4096;           // staging of one output warp: 32 rows x 128 bytes
 constexpr int kGlThreads = 192;
 constexpr int kGlLong = 8;                   // stages between additions to the total
 
 constexpr int gl_stage_bytes(int bn, int ctas) { return kGlABytes + bn / ctas * 128; }
 constexpr int gl_stages(int bn, int ctas) { return gl_stage_bytes(bn, ctas) > 32768 ? 4 : gl_stage_bytes(bn, ctas) > 24576 ? 6 : 8; }
 constexpr int gl_smem(int bn, int ctas) {  // alignment, ring, staging, bias per output warp, barriers
-    return 1024 + gl_stages(bn, ctas) * gl_stage_bytes(bn, ctas) + 4 * kGlStageWarp + 4 * bn * 4 + 256;
+    return 1024 + gl_stages(bn, ctas) * gl_stage_bytes(bn, ctas) + 4 * kStagingBytes + 4 * bn * 4 + 256;
 }
 
 struct GlArgs {
     GroupPlanView plan;
-    void* out;
+    RowsOut o;
     void* sums;              // dw: dbias, or null
     const float* tile_sums;  // dw: sums of dy's columns per tile of 128 rows [tiles][N]
     const void* bias;        // forward, or null
-    int64_t ld_out;          // elements
-    int32_t out_type, sums_type, bias_type;
+    int32_t sums_type, bias_type;
     int32_t T, E, N;         // N: rows of w per bucket
-    int32_t red, cols;       // length of the reduction (forward, dx); columns of the output
+    int32_t red;             // length of the reduction (forward, dx)
     int32_t col_tiles;       // ceil(cols / BN)
     int32_t row_tiles;       // dw: tiles along N
     int32_t gather;          // forward, dx: A's rows are gathered by the plan's order
-    int32_t vec;             // rows of `out` start at multiples of 16 bytes
     uint32_t idesc;
     unsigned long long* status;
 };
@@ -109,72 +105,15 @@ __device__ __forceinline__ int gl_steps(const GlArgs& a, const GlTile& x, int c)
     return left >= kGlK ? 4 : (left + 15) >> 4;
 }
 
-// Position in the ring of stages.
-template <int S>
-struct GlRing {
-    int stage = 0;
-    unsigned phase = 0;
-    __device__ __forceinline__ void next() {
-        if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-        }
-    }
-};
-
-// A pass of columns (`bytes` per row in the warp's staging, 16-byte pieces swizzled) to the rows of the output, in whole
-// 128- or 64-byte pieces of rows.  Lane r holds row r's place in the output, or -1.
-__device__ __forceinline__ void gl_copy_out(const GlArgs& a, const unsigned char* stg, int bytes, int32_t my_row, int64_t row_base,
-                                            int col) {
-    const int lane = threadIdx.x & 31;
-    const int es = a.out_type == NNUE_T_F32 ? 4 : 2;
-    unsigned char* out = static_cast<unsigned char*>(a.out);
-    __syncwarp();
-    if (a.vec) {
-        const int shift = bytes == 128 ? 3 : 2, piece = lane & ((1 << shift) - 1);
-        const bool inside = col + piece * (16 / es) < a.cols;  // cols is a multiple of a piece
-#pragma unroll
-        for (int it = 0; it < 8; ++it) {
-            const int r = (it << (5 - shift)) + (lane >> shift);
-            const int32_t row = __shfl_sync(kFullMask, my_row, r & 31);
-            if (r >= 32 || row < 0 || !inside) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
-            *reinterpret_cast<uint4*>(out + ((row_base + row) * a.ld_out + col) * es + piece * 16) = v;
-        }
-    } else {
-#pragma unroll 1
-        for (int r = 0; r < 32; ++r) {
-            const int32_t row = __shfl_sync(kFullMask, my_row, r);
-            if (row < 0) continue;
-            for (int j = lane; j < bytes / es && col + j < a.cols; j += 32) {
-                const unsigned char* src = stg + r * 128 + (((j * es / 16) ^ (r & 7)) << 4) + j * es % 16;
-                unsigned char* dst = out + ((row_base + row) * a.ld_out + col + j) * es;
-                if (es == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-                else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
-            }
-        }
-    }
-    __syncwarp();
-}
-
-__device__ __forceinline__ uint32_t pack_half(float a, float b, int32_t type) {
-    if (type == NNUE_T_BF16) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&v);
-    }
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 // One output warp: its 32 rows of the tile, from tensor memory (or zeros) to the output.
 template <int BN>
 __device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bool zeros, const float* s_bias, unsigned char* stg,
                                              int32_t my_row, int64_t row_base, int col0) {
     const int lane = threadIdx.x & 31;
-    const bool f32 = a.out_type == NNUE_T_F32;
+    const bool f32 = a.o.type == NNUE_T_F32;
     const bool wide = !f32 && BN >= 64;  // two reads of 32 columns make one 128-byte piece of a row
 #pragma unroll 1
-    for (int c = 0; c < BN && col0 + c < a.cols; c += wide ? 64 : 32) {
+    for (int c = 0; c < BN && col0 + c < a.o.cols; c += wide ? 64 : 32) {
 #pragma unroll 1
         for (int h = 0; h < (wide ? 2 : 1); ++h) {
             uint32_t v[32];
@@ -206,12 +145,12 @@ __device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bo
                     uint32_t w[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        w[j] = pack_half(__uint_as_float(v[8 * p + 2 * j]), __uint_as_float(v[8 * p + 2 * j + 1]), a.out_type);
+                        w[j] = pack_half(__uint_as_float(v[8 * p + 2 * j]), __uint_as_float(v[8 * p + 2 * j + 1]), a.o.type);
                     *reinterpret_cast<uint4*>(stg + lane * 128 + (((4 * h + p) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
-        gl_copy_out(a, stg, f32 || wide ? 128 : 64, my_row, row_base, col0 + c);
+        copy_rows_out(a.o, stg, f32 || wide ? 128 : 64, my_row, row_base, col0 + c);
     }
 }
 
@@ -222,7 +161,7 @@ __device__ __forceinline__ bool gl_copy_role(const GlArgs& a, const CUtensorMap*
     constexpr bool PAIR = CTAS == 2;
     constexpr int S = gl_stages(BN, CTAS), kBn = BN / CTAS;  // kBn: this CTA's columns of B
     const int lane = threadIdx.x & 31;
-    GlRing<S> at;
+    StageRing<S> at;
     bool ok = true;
     for (int t = t0; t < tiles && ok; t += stride) {
         const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
@@ -231,16 +170,16 @@ __device__ __forceinline__ bool gl_copy_role(const GlArgs& a, const CUtensorMap*
         // blocks of 64 columns wholly outside the operand are not read: their rows or columns of D are never stored
         const int a_row0 = x.row0 + side * kGroupRows, b_col0 = x.col0 + side * kBn;
         const int a_boxes = MODE == kModeDw ? max(0, min(2, (a.N - a_row0 + 63) >> 6)) : 0;
-        const int b_boxes = MODE == kModeFwd ? 0 : max(0, min(kBn / 64, (a.cols - b_col0 + 63) >> 6));
+        const int b_boxes = MODE == kModeFwd ? 0 : max(0, min(kBn / 64, (a.o.cols - b_col0 + 63) >> 6));
         const bool a_rows = MODE != kModeDw && x.count > side * kGroupRows;
         const bool gather = MODE != kModeDw && !PAIR && a.gather;
         // the bytes that complete the stage: both CTAs' of a pair, announced by the first
         int bytes;
         if (MODE == kModeDw) {
-            bytes = (min(2 * CTAS, (a.N - x.row0 + 63) >> 6) + min(BN / 64, (a.cols - x.col0 + 63) >> 6)) * kGlBoxBytes;
+            bytes = (min(2 * CTAS, (a.N - x.row0 + 63) >> 6) + min(BN / 64, (a.o.cols - x.col0 + 63) >> 6)) * kGlBoxBytes;
         } else {
             bytes = gather ? ((x.count + 3) >> 2) * 512 : (PAIR && x.count > kGroupRows ? 2 : 1) * kGlABytes;
-            bytes += MODE == kModeFwd ? BN * 128 : min(BN / 64, (a.cols - x.col0 + 63) >> 6) * kGlBoxBytes;
+            bytes += MODE == kModeFwd ? BN * 128 : min(BN / 64, (a.o.cols - x.col0 + 63) >> 6) * kGlBoxBytes;
         }
         int rows[4];
         if (gather) {
@@ -285,8 +224,8 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
     constexpr bool PAIR = CTAS == 2;
     constexpr bool kAMn = MODE == kModeDw, kBMn = MODE != kModeFwd;
     constexpr uint32_t kAStep = kAMn ? 2048 >> 4 : 32 >> 4, kBStep = kBMn ? 2048 >> 4 : 32 >> 4;  // 16 reduction elements
-    GlRing<gl_stages(BN, CTAS)> at;
-    GlRing<2> acc;
+    StageRing<gl_stages(BN, CTAS)> at;
+    StageRing<2> acc;
     bool ok = true;
     for (int t = t0; t < tiles && ok; t += stride) {
         const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
@@ -362,7 +301,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
     unsigned char* staging = ring_ptr + S * gl_stage_bytes(BN, CTAS);
-    float* s_bias = reinterpret_cast<float*>(staging + 4 * kGlStageWarp);  // [4][BN], one copy per output warp
+    float* s_bias = reinterpret_cast<float*>(staging + 4 * kStagingBytes);  // [4][BN], one copy per output warp
     uint64_t* full = reinterpret_cast<uint64_t*>(s_bias + 4 * BN);         // [S] a stage's copies are in (pair: the first CTA's)
     uint64_t* empty = full + S;                                            // [S] a stage may be overwritten
     uint64_t* done = empty + S;                                            // [2] an accumulator is complete
@@ -413,7 +352,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
         const int q = warp & 3;  // the quarter of tensor memory's lanes that this warp may read
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         float* my_bias = s_bias + q * BN;
-        GlRing<2> acc;
+        StageRing<2> acc;
         for (int t = t0; t < tiles && ok; t += stride) {
             const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
             const bool some = x.c1 > x.c0;
@@ -430,7 +369,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
             const bool biased = MODE == kModeFwd && !SPLIT && a.bias && x.live;
             if (biased) {
                 for (int j = lane; j < BN; j += 32)
-                    my_bias[j] = x.col0 + j < a.cols ? load_as_float(a.bias, a.bias_type, (int64_t)x.bucket * a.N + x.col0 + j) : 0.f;
+                    my_bias[j] = x.col0 + j < a.o.cols ? load_as_float(a.bias, a.bias_type, (int64_t)x.bucket * a.N + x.col0 + j) : 0.f;
                 __syncwarp();
             }
             auto give_back = [&] {
@@ -458,7 +397,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
             }
             if (!ok || SPLIT) break;
             if (__any_sync(kFullMask, my_row >= 0))
-                gl_bring_out<BN>(a, from, !some, biased ? my_bias : nullptr, staging + q * kGlStageWarp, my_row, row_base, x.col0);
+                gl_bring_out<BN>(a, from, !some, biased ? my_bias : nullptr, staging + q * kStagingBytes, my_row, row_base, x.col0);
             if (!LONG && some) give_back();
         }
     }
@@ -490,10 +429,10 @@ __global__ void __launch_bounds__(kGlThreads, 1)
         // row r of the tile is finished by rank r mod ranks: partial sums in the order of the ranks
         const int rows = MODE == kModeDw ? min(kGroupRows, a.N - x.row0) : x.count;
         const int mine = (rows - rank + ranks - 1) / ranks;
-        const int es = a.out_type == NNUE_T_F32 ? 4 : 2;
+        const int es = a.o.type == NNUE_T_F32 ? 4 : 2;
         for (int i = tid; i < mine * (BN / 4); i += kGlThreads) {
             const int r = rank + i / (BN / 4) * ranks, c = i % (BN / 4) * 4, col = x.col0 + c;
-            if (col >= a.cols) continue;
+            if (col >= a.o.cols) continue;
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             if (x.live) {
                 const uint32_t addr = ring + (uint32_t)(r * kPartPitch + c) * 4;
@@ -508,19 +447,19 @@ __global__ void __launch_bounds__(kGlThreads, 1)
             if (MODE == kModeFwd && a.bias && x.live) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (col + j < a.cols) v[j] += load_as_float(a.bias, a.bias_type, (int64_t)x.bucket * a.N + col + j);
+                    if (col + j < a.o.cols) v[j] += load_as_float(a.bias, a.bias_type, (int64_t)x.bucket * a.N + col + j);
             }
             const int64_t row = MODE == kModeDw ? (int64_t)x.bucket * a.N + x.row0 + r : (int64_t)__ldg(a.plan.order + x.first + r);
-            const int64_t at = row * a.ld_out + col;
-            if (a.vec && es == 4) {
-                *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-            } else if (a.vec) {
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
-                    make_uint2(pack_half(v[0], v[1], a.out_type), pack_half(v[2], v[3], a.out_type));
+            const int64_t at = row * a.o.ld + col;
+            if (a.o.vec && es == 4) {
+                *reinterpret_cast<float4*>(static_cast<float*>(a.o.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+            } else if (a.o.vec) {
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o.out) + at) =
+                    make_uint2(pack_half(v[0], v[1], a.o.type), pack_half(v[2], v[3], a.o.type));
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (col + j < a.cols) store_from_float(a.out, a.out_type, at + j, v[j]);
+                    if (col + j < a.o.cols) store_from_float(a.o.out, a.o.type, at + j, v[j]);
             }
         }
         if (MODE == kModeDw && a.sums && x.col0 == 0 && rank == 0 && tid < rows) gl_bias_gradient(a, x, x.row0 + tid);
@@ -533,10 +472,6 @@ __global__ void __launch_bounds__(kGlThreads, 1)
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-struct GlShape {
-    int bn, ctas, ranks;
-};
-
 template <int MODE, int BN, int CTAS, bool SPLIT, bool LONG>
 int gl_launch(const CUtensorMap& ma, const CUtensorMap& mb, const GlArgs& a, int64_t tiles, int ranks, cudaStream_t s) {
     auto kernel = k_grouped<MODE, BN, CTAS, SPLIT, LONG>;
@@ -567,25 +502,10 @@ int gl_launch(const CUtensorMap& ma, const CUtensorMap& mb, const GlArgs& a, int
     return NNUE_OK;
 }
 
-// Width of a tile, CTAs on it and parts of its sum.  `rows` per bucket in use and the number of such runs of rows are
-// estimates in forward and dx (the host does not know the plan), exact in dw; `chunks` is the length of the reduction in
-// stages.  Pairs where they fill the GPU.  Else the widest tile that still gives every SM one; where even the narrowest
-// leaves SMs idle, the sum is split while every part keeps two stages.
-static GlShape gl_shape(int64_t runs, int64_t rows, int64_t cols, int64_t chunks, int narrowest, int widest, bool pairs) {
-    const int64_t sms = sm_count();
-    auto tiles = [&](int64_t high, int64_t wide) { return runs * ((rows + high - 1) / high) * ((cols + wide - 1) / wide); };
-    if (pairs && rows > kGroupRows && tiles(kGroupPairRows, widest) * 2 >= sms) return {widest, 2, 1};
-    int bn = widest;
-    while (bn > narrowest && (tiles(kGroupRows, bn) < sms || cols <= bn / 2)) bn /= 2;
-    int ranks = 1;
-    while (ranks < 8 && tiles(kGroupRows, bn) * ranks * 2 <= sms && chunks >= ranks * 4) ranks *= 2;
-    return {bn, 1, ranks};
-}
-
 template <int MODE, bool LONG>
-int gl_run(const CUtensorMap& ma, const CUtensorMap& mb, GlArgs& a, int64_t tile_rows, GlShape shape, cudaStream_t s) {
+int gl_run(const CUtensorMap& ma, const CUtensorMap& mb, GlArgs& a, int64_t tile_rows, TileShape shape, cudaStream_t s) {
     constexpr int kNarrowest = MODE == kModeFwd ? 32 : 64, kWidest = LONG ? 128 : 256;
-    a.col_tiles = (a.cols + shape.bn - 1) / shape.bn;
+    a.col_tiles = (a.o.cols + shape.bn - 1) / shape.bn;
     a.idesc = umma_idesc(a.idesc, (uint32_t)(kGroupRows * shape.ctas), (uint32_t)shape.bn, MODE == kModeDw, MODE != kModeFwd);
     const int64_t tiles = tile_rows * a.col_tiles;
     NNUE_REQUIRE(tiles * 8 < 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "grouped linear: too many tiles");
@@ -647,15 +567,11 @@ static int common_args(const char* what, GlArgs* a, const void* plan, int64_t T,
                        int32_t out_type, int64_t cols) {
     *a = GlArgs{};
     a->plan = group_view(plan, T, E);
-    a->out = out;
-    a->ld_out = cols;
-    a->out_type = out_type;
+    a->o = rows_out(out, out_type, cols);
     a->T = (int32_t)T;
     a->E = E;
     a->N = (int32_t)N;
-    a->cols = (int32_t)cols;
     a->row_tiles = 1;
-    a->vec = cols * type_bytes(out_type) % 16 == 0;
     a->idesc = type == NNUE_T_BF16 ? 1u : 0u;  // the operands' format; the rest of the descriptor follows the tile
     a->status = device_status_ptr();
     NNUE_REQUIRE(a->status, NNUE_ERR_CUDA, "%s: no device status word", what);
@@ -685,7 +601,7 @@ extern "C" int nnue_grouped_linear_fwd(const void* x, int64_t ldx, int32_t laid,
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("grouped_fwd", s);
     const int64_t runs = E < T ? E : T;
-    const GlShape shape = gl_shape(runs, (T + runs - 1) / runs, N, (K + kGlK - 1) / kGlK, 32, 256, laid);
+    const TileShape shape = tile_shape(runs, (T + runs - 1) / runs, N, (K + kGlK - 1) / kGlK, 32, 256, laid);
     CUtensorMap ma, mb;
     if (int st = operand_map(&ma, &a, laid, x, ldx, T, K, E, type)) return st;
     if (int st = weight_map(&mb, w, ldw, E, N, K, shape.bn / shape.ctas, type)) return st;
@@ -706,7 +622,7 @@ extern "C" int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, int32
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("grouped_dx", s);
     const int64_t runs = E < T ? E : T;
-    const GlShape shape = gl_shape(runs, (T + runs - 1) / runs, K, (N + kGlK - 1) / kGlK, 64, 256, laid);
+    const TileShape shape = tile_shape(runs, (T + runs - 1) / runs, K, (N + kGlK - 1) / kGlK, 64, 256, laid);
     CUtensorMap ma, mb;
     if (int st = operand_map(&ma, &a, laid, dy, lddy, T, N, E, type)) return st;
     if (int st = weight_map(&mb, w, ldw, E, N, K, 64, type)) return st;
@@ -735,7 +651,7 @@ extern "C" int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_su
     ProfScope prof("grouped_dw", s);
     const bool fp32 = dw_type == NNUE_T_F32;
     const int64_t mean = (T + E - 1) / E;
-    const GlShape shape = gl_shape(E, N, K, (mean + kGlK - 1) / kGlK, 64, fp32 ? 128 : 256, true);
+    const TileShape shape = tile_shape(E, N, K, (mean + kGlK - 1) / kGlK, 64, fp32 ? 128 : 256, true);
     a.row_tiles = (int32_t)((N + kGroupRows * shape.ctas - 1) / (kGroupRows * shape.ctas));
     CUtensorMap ma, mb;
     if (T > 0) {

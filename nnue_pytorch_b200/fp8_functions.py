@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._launch import _ptr, _require_cuda, _span, _stream
-from .grouped_linear_functions import TYPES, GroupPlan, _on, _pitched
+from .grouped_linear_functions import GATHERED_ROWS, TYPES, GroupPlan, _on, _pitched
 
 FORMATS = (torch.float8_e4m3fn, torch.float8_e5m2)
 BLOCK = 128
@@ -86,7 +86,7 @@ def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn
     scale = torch.empty(T, (K + BLOCK - 1) // BLOCK, dtype=torch.float32, device=dev)
     with _on(dev), _span("fp8_rows", dev):
         st = _lib.load().nnue_fp8_quantize_rows(_ptr(x), TYPES[x.dtype], ldx, _ptr(q), ldq, _ptr(scale), T, K, TYPES[format],
-                                                _stream(dev))
+                                                None, 0, _stream(dev))
     _lib.check(st, "nnue_fp8_quantize_rows")
     return Fp8Blocks(q, scale)
 
@@ -127,34 +127,53 @@ def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tenso
         (isinstance(x, torch.Tensor) and x.requires_grad) or (bias is not None and bias.requires_grad)), \
         "linear_fp8 has no gradient: call it under torch.no_grad()"
     format = weight.q.dtype
-    if isinstance(x, torch.Tensor):
-        out_dtype = out_dtype or x.dtype
-        _require_cuda(x, weight.q)
-        x = quantize_fp8_rows(x, format)
-    assert x.scale.dim() == 2 and x.q.dtype == format, "the rows are Fp8Blocks of rows in the weight's format"
-    out_dtype = out_dtype or torch.bfloat16
-    assert out_dtype in (torch.float32, torch.bfloat16, torch.float16)
-    dev = _require_cuda(x.q, x.scale, weight.q, weight.scale) if bias is None else \
-        _require_cuda(x.q, x.scale, weight.q, weight.scale, bias)
     E = weight.scale.shape[0]
-    T, K = x.q.shape
+    given = not isinstance(x, torch.Tensor)
+    if given:
+        assert x.scale.dim() == 2 and x.q.dtype == format, "the rows are Fp8Blocks of rows in the weight's format"
+        rows, out_dtype = x.q, out_dtype or torch.bfloat16
+    else:
+        _check_source(x, format)
+        rows, out_dtype = x, out_dtype or x.dtype
+    assert out_dtype in (torch.float32, torch.bfloat16, torch.float16)
+    dev = _require_cuda(rows, weight.q, weight.scale)
+    if given:
+        _require_cuda(rows, x.scale)
+    T, K = rows.shape
     N = weight.q.shape[0] // E
     assert weight.q.shape[1] == K, f"rows of {K} inputs against weights of {weight.q.shape[1]}"
     if plan is not None:
-        plan.check(x.q)
+        plan.check(rows)
         assert plan.count == E, f"a plan of {plan.count} buckets for {E} matrices"
     else:
         assert E == 1, "several matrices need a plan"
     if bias is not None:
+        _require_cuda(rows, bias)
         assert bias.dtype == torch.float32 and bias.numel() == E * N
         bias = bias.detach().contiguous()
     lib = _lib.load()
+    laid = plan is not None and T > GATHERED_ROWS * E  # few rows per bucket are gathered by the product itself
+    buffer = None if plan is None else _ptr(plan.buffer)
     y = torch.empty(T, N, dtype=out_dtype, device=dev)
     with _on(dev), _span("linear_fp8", dev):
-        xr, ldx = _pitched(x.q, format, lib, dev)
+        s = _stream(dev)
         wr, ldw = _pitched(weight.q, format, lib, dev)
-        st = lib.nnue_fp8_linear_fwd(_ptr(xr), ldx, _ptr(x.scale), _ptr(wr), ldw, _ptr(weight.scale), _ptr(bias),
-                                     None if plan is None else _ptr(plan.buffer), _ptr(y), TYPES[out_dtype], T, K, N, E,
-                                     TYPES[format], _stream(dev))
+        if not given and not laid:
+            x = quantize_fp8_rows(x, format)
+        if not given and laid:
+            xs, ldx = _source(x)
+            xr = torch.empty(lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E), dtype=torch.uint8, device=dev)
+            scale = torch.empty(T, (K + BLOCK - 1) // BLOCK, dtype=torch.float32, device=dev)
+            _lib.check(lib.nnue_fp8_quantize_rows(_ptr(xs), TYPES[xs.dtype], ldx, _ptr(xr), 0, _ptr(scale), T, K, TYPES[format],
+                                                  buffer, E, s), "nnue_fp8_quantize_rows")
+        else:
+            scale = x.scale
+            xr, ldx = _pitched(x.q, format, lib, dev, whole=laid)
+            if laid:  # pairs of bytes as 16-bit numbers, moved as they are
+                src, xr = xr, torch.empty(lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E), dtype=torch.uint8, device=dev)
+                _lib.check(lib.nnue_group_rows(_ptr(src), TYPES[torch.bfloat16], ldx // 2, buffer, _ptr(xr), TYPES[torch.bfloat16],
+                                               None, T, (K + 15) // 16 * 8, E, s), "nnue_group_rows")
+        st = lib.nnue_fp8_linear_fwd(_ptr(xr), ldx, laid, _ptr(scale), _ptr(wr), ldw, _ptr(weight.scale), _ptr(bias), buffer,
+                                     _ptr(y), TYPES[out_dtype], T, K, N, E, TYPES[format], s)
     _lib.check(st, "nnue_fp8_linear_fwd")
     return y

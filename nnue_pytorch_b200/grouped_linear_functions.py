@@ -75,12 +75,14 @@ class GroupPlan:
         assert t.device == self.device, "the plan lives on another device"
 
 
-def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev) -> tuple[torch.Tensor, int]:
+def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev, whole: bool = False) -> tuple[torch.Tensor, int]:
     """(t as rows of `dtype` that start at multiples of 16 bytes, their pitch in elements): `t` itself where it is one,
-    else a copy whose rows are padded with zeros (`nnue_pack_rows`)."""
+    else a copy whose rows are padded with zeros (`nnue_pack_rows`).  `whole`: the last 16 bytes of every row may be read."""
     rows, cols = t.shape
     unit = 16 // dtype.itemsize
-    if t.dtype == dtype and (cols == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0:
+    if whole and cols % unit:
+        pass
+    elif t.dtype == dtype and (cols == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0:
         pitch = t.stride(0)
         if pitch % unit == 0 and pitch >= cols:
             return t, pitch

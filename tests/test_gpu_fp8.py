@@ -144,39 +144,44 @@ def _linear(dev, T, count, K, N, format, out_dtype, seed, arbitrary_scales=False
 
 @pytest.mark.parametrize("format", FORMATS)
 @pytest.mark.parametrize("T,count,K,N", [(1, 1, 16, 1), (1, 8, 128, 64), (2, 3, 40, 7), (130, 1, 129, 129), (300, 5, 512, 200),
-                                         (64, 70, 200, 33), (1000, 8, 1024, 32), (257, 2, 1000, 300), (4, 2, 4100, 130)])
+                                         (64, 70, 200, 33), (1000, 8, 1024, 32), (257, 2, 1000, 300), (4, 2, 4100, 130),
+                                         (9000, 8, 300, 2100), (20000, 3, 1000, 520), (5000, 40, 130, 520)])
 def test_linear(dev, T, count, K, N, format):
-    for i, out in enumerate((torch.bfloat16, torch.float16, torch.float32)):
+    for i, out in enumerate((torch.bfloat16, torch.float16, torch.float32) if T < 5000 else (torch.bfloat16,)):
         _linear(dev, T, count, K, N, format, out, T + i)
     _linear(dev, T, count, K, N, format, torch.float32, T + 5, arbitrary_scales=True)
     _linear(dev, T, 1, K, N, format, torch.float32, T + 6, dense=True)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-def test_linear_quantises_its_rows(dev, dtype):
+@pytest.mark.parametrize("T,K", [(77, 200), (30, 200), (900, 208), (900, 1030)])
+def test_linear_quantises_its_rows(dev, dtype, T, K):
     from nnue_pytorch_b200 import GroupPlan, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
 
     g = torch.Generator().manual_seed(2)
-    x = torch.randn(77, 200, generator=g).to(dev, dtype)
-    w8 = quantize_fp8_tiles(torch.randn(3 * 50, 200, generator=g).to(dev), 3)
-    plan = GroupPlan(torch.randint(-1, 3, (77,), generator=g).to(dev), 3)
+    x = torch.randn(T, K, generator=g).to(dev, dtype)
+    w8 = quantize_fp8_tiles(torch.randn(3 * 50, K, generator=g).to(dev), 3)
+    plan = GroupPlan(torch.randint(-1, 3, (T,), generator=g).to(dev), 3)
     y = linear_fp8(x, w8, None, plan)
     assert y.dtype == dtype
     assert torch.equal(y, linear_fp8(quantize_fp8_rows(x), w8, None, plan, dtype))
     assert torch.equal(y, linear_fp8(x, w8, None, plan))  # the same bits again
-    wide = torch.randn(77, 400, generator=g).to(dev, dtype)
-    assert torch.equal(linear_fp8(wide[:, 1:401:2], w8, None, plan), linear_fp8(wide[:, 1:401:2].contiguous(), w8, None, plan))
+    wide = torch.randn(T, 2 * K, generator=g).to(dev, dtype)
+    assert torch.equal(linear_fp8(wide[:, 1::2], w8, None, plan), linear_fp8(wide[:, 1::2].contiguous(), w8, None, plan))
+    assert torch.equal(linear_fp8(wide[:, 3 : 3 + K], w8, None, plan), linear_fp8(wide[:, 3 : 3 + K].contiguous(), w8, None, plan))
 
 
 def test_linear_with_unaligned_operands(dev):
-    from nnue_pytorch_b200 import Fp8Blocks, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
+    from nnue_pytorch_b200 import Fp8Blocks, GroupPlan, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
 
     g = torch.Generator().manual_seed(5)
     x8 = quantize_fp8_rows(torch.randn(40, 130, generator=g).to(dev))
     w8 = quantize_fp8_tiles(torch.randn(30, 130, generator=g).to(dev))
     want = linear_fp8(x8, w8)
+    plan = GroupPlan(torch.randint(-1, 1, (40,), generator=g).to(dev), 1)
     tight = lambda q: q.view(torch.uint8).contiguous().view(q.dtype)  # noqa: E731  rows of 130 bytes
     assert torch.equal(want, linear_fp8(Fp8Blocks(tight(x8.q), x8.scale), Fp8Blocks(tight(w8.q), w8.scale)))
+    assert torch.equal(linear_fp8(x8, w8, None, plan), linear_fp8(Fp8Blocks(tight(x8.q), x8.scale), w8, None, plan))
 
 
 def test_not_finite_rows(dev):
