@@ -797,16 +797,17 @@ int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_sums,
  * Numbers that are not finite become NaN in E4M3 and stay what they are in E5M2.
  * rows:  x [T, K] (F32, BF16 or F16, pitch ldx) -> q [T, K] (pitch ldq, at most
  *        the row length rounded up to 128; columns [K, ldq) become zero),
- *        scale [T, ceil(K / 128)].  With a plan (of T rows and E buckets) q's rows
+ *        scale [T, ceil(K / 128)], or with scale_ld > 0 [ceil(K / 128), scale_ld] by
+ *        the rows' places in q.  With a plan (of T rows and E buckets) q's rows
  *        are laid out by bucket as nnue_group_rows lays them, at a pitch of K rounded
  *        up to 16 (ldq is not looked at), and what lies between buckets is left as it
- *        is; scale stays in the batch's order, and rows without a bucket get none.
+ *        is; rows without a bucket get no scale.
  * tiles: w [E, N, K] (pitch ldw) -> q [E, N, K], scale [E, ceil(N / 128),
  *        ceil(K / 128)]; tiles start anew in every bucket. */
 int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, void* q,
-                           int64_t ldq, float* scale, int64_t T, int64_t K,
-                           int32_t format, const void* plan, int32_t E,
-                           void* stream);
+                           int64_t ldq, float* scale, int64_t scale_ld,
+                           int64_t T, int64_t K, int32_t format,
+                           const void* plan, int32_t E, void* stream);
 int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
                             int64_t ldq, float* scale, int32_t E, int64_t N,
                             int64_t K, int32_t format, void* stream);
@@ -814,13 +815,13 @@ int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
 /* y[p, n] = sum_c x_scale[p, c] w_scale[b, n / 128, c]
  *                 sum_{k in block c} x[p, k] w[b, n, k]  + bias[b, n]
  * x [T, K] and w [E, N, K] of one 8-bit format, pitches that are multiples of 16,
- * scales as the quantisers lay them out (any fp32 values, not only powers of
- * two), bias [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are
+ * scales as the quantisers lay them out (x_scale with the same scale_ld; by place
+ * with rows laid out by bucket or one matrix; any fp32 values, not only powers of two), bias [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are
  * fp32.  plan NULL: E = 1 and every row belongs to the one matrix.  With a plan, x
  * is laid out by bucket (`laid`; ldx is not looked at) or in the batch's order,
  * which suits a few rows per bucket. */
 int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid,
-                        const float* x_scale,
+                        const float* x_scale, int64_t scale_ld,
                         const void* w, int64_t ldw, const float* w_scale,
                         const float* bias, const void* plan, void* y,
                         int32_t y_type, int64_t T, int64_t K, int64_t N,

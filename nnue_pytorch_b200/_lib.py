@@ -243,11 +243,11 @@ PROTOTYPES = {
     ),
     "nnue_grouped_linear_bwd_input": (C.c_int, [_P, _I64, _I32, _P, _I64, _P, _P, _I64, _I64, _I64, _I32, _I32, _P]),
     "nnue_grouped_linear_bwd_weight": (C.c_int, [_P, _P, _P, _P, _P, _I32, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P]),
-    "nnue_fp8_quantize_rows": (C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I64, _I64, _I32, _P, _I32, _P]),
+    "nnue_fp8_quantize_rows": (C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I32, _P]),
     "nnue_fp8_quantize_tiles": (C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I32, _I64, _I64, _I32, _P]),
     "nnue_fp8_linear_fwd": (
         C.c_int,
-        [_P, _I64, _I32, _P, _P, _I64, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P],
+        [_P, _I64, _I32, _P, _I64, _P, _I64, _P, _P, _P, _P, _I32, _I64, _I64, _I64, _I32, _I32, _P],
     ),
     "nnue_batch_build_halfka": (C.c_int, [_P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }

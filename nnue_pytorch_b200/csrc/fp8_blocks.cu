@@ -138,6 +138,7 @@ struct Fp8Args {
     uint8_t* q;
     float* scale;
     int64_t ldx, ldq, T;
+    int64_t scale_ld;     // 0: scale [T, C]; else [C, scale_ld] by places in q
     int32_t K, type, format, E;
     int32_t warps;        // per row: four blocks each
     int32_t vec_x, vec_q;
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) k_fp8_rows(const __grid_constant__ F
     const int e = fp8_scale_exponent(most, a.format);
     store_sixteen(a.q, to * a.ldq + k, (int)min((int64_t)kLaneNumbers, a.ldq - k), a.vec_q, v, power_of_two(-e), a.format);
     const int c = k / kFp8Block;
-    if (lane % kBlockLanes == 0 && c < C) a.scale[from * C + c] = power_of_two(e);
+    if (lane % kBlockLanes == 0 && c < C) a.scale[a.scale_ld ? c * a.scale_ld + to : from * C + c] = power_of_two(e);
 }
 
 // One CTA per 128 x 128 tile: every number is read once and held in registers, 64 per thread, until the scale is known.
@@ -222,7 +223,7 @@ static int check_fp8(const char* what, const void* x, int32_t type, int64_t ldx,
     return NNUE_OK;
 }
 
-extern "C" int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t T,
+extern "C" int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, void* q, int64_t ldq, float* scale, int64_t scale_ld, int64_t T,
                                       int64_t K, int32_t format, const void* plan, int32_t E, void* stream) {
     const char* what = "nnue_fp8_quantize_rows";
     if (plan) {
@@ -231,6 +232,7 @@ extern "C" int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, 
     }
     if (int st = check_fp8(what, x, type, ldx, q, ldq, scale, T, K, format)) return st;
     NNUE_REQUIRE(K < (1 << 24), NNUE_ERR_UNSUPPORTED, "%s: rows of %lld numbers", what, (long long)K);
+    NNUE_REQUIRE(scale_ld == 0 || scale_ld >= (plan ? group_laid_rows(T, E) : T), NNUE_ERR_ARG, "%s: no room for every row's scales", what);
     if (T == 0) return NNUE_OK;
     Fp8Args a = {};
     if (plan) a.plan = group_view(plan, T, E);
@@ -239,6 +241,7 @@ extern "C" int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, 
     a.scale = scale;
     a.ldx = ldx;
     a.ldq = ldq;
+    a.scale_ld = scale_ld;
     a.T = T;
     a.K = (int32_t)K;
     a.type = type;

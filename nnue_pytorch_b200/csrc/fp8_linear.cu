@@ -17,7 +17,11 @@ namespace nnue {
 
 constexpr int kF8K = 128;
 constexpr int kF8ABytes = kGroupRows * 128;
-constexpr int kF8Threads = 320;
+constexpr int kF8Threads = 384;  // copies, instructions, two warps without work, eight output warps
+constexpr int kF8OutWarp = 4;    // the first output warp
+// An output thread of the widest tile holds 128 sums and two reads of 32 columns: the first warpgroup gives registers up.
+constexpr int kF8FewRegs = 56, kF8ManyRegs = 224, kF8LaunchRegs = 168;
+static_assert(128 * kF8FewRegs + 256 * kF8ManyRegs <= kF8Threads * kF8LaunchRegs, "more registers than the launch brings");
 
 constexpr int f8_stage_bytes(int bn, int ctas) { return kF8ABytes + bn / ctas * 128; }
 constexpr int f8_stages(int bn, int ctas) { return f8_stage_bytes(bn, ctas) > 32768 ? 4 : f8_stage_bytes(bn, ctas) > 24576 ? 6 : 8; }
@@ -28,6 +32,7 @@ struct F8Args {
     GroupPlanView plan;
     RowsOut o;
     const float *x_scale, *w_scale, *bias;
+    int64_t scale_ld;    // 0: x_scale [T, C] by rows of the batch; else [C, scale_ld] by the rows' places in x
     int32_t T, E, N, K;
     int32_t C, R;        // blocks along K and along N
     int32_t col_tiles;
@@ -147,13 +152,191 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
 }
 
+// Scales of four consecutive stages of one thread: its row's and its columns'.
+struct F8Scales {
+    float x[4], w[4];
+};
+struct F8ScaleAt {
+    const float *x, *w;
+    int64_t step;  // of x from one block to the next
+    int32_t end;
+};
+__device__ __forceinline__ F8ScaleAt f8_scale_at(const F8Args& a, const F8Tile& x, int r, int col) {
+    F8ScaleAt s;
+    const bool mine = r < x.count;
+    if (a.scale_ld) {
+        s.x = a.x_scale + (mine ? x.place + r : 0);
+        s.step = a.scale_ld;
+    } else {
+        const int row = !mine ? 0 : a.dense ? x.first + r : __ldg(a.plan.order + x.first + r);
+        s.x = a.x_scale + (int64_t)row * a.C;
+        s.step = 1;
+    }
+    s.w = a.w_scale + ((int64_t)(x.live ? x.bucket : 0) * a.R + min(col / kF8K, a.R - 1)) * a.C;
+    s.end = mine ? x.c1 : 0;
+    return s;
+}
+__device__ __forceinline__ void f8_load_scale(const F8ScaleAt& s, int c, float& x, float& w) {
+    x = w = 0.f;
+    if (c < s.end) {
+        x = __ldg(s.x + c * s.step);
+        w = __ldg(s.w + c);
+    }
+}
+
+// An output warp's 32 rows and half of the columns, from registers to the output.
+template <int HALF>
+__device__ __forceinline__ void f8_bring_out(const F8Args& a, const F8Tile& x, float (&acc)[HALF], unsigned char* stg, int32_t my_row,
+                                             int col) {
+    const int lane = threadIdx.x & 31;
+    if (a.bias && x.live) {
+        float* b = reinterpret_cast<float*>(stg);
+        for (int j = lane; j < HALF; j += 32) b[j] = col + j < a.o.cols ? __ldg(a.bias + (int64_t)x.bucket * a.N + col + j) : 0.f;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < HALF; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(b + j);
+            acc[j] += v.x;
+            acc[j + 1] += v.y;
+            acc[j + 2] += v.z;
+            acc[j + 3] += v.w;
+        }
+        __syncwarp();
+    }
+    if (a.o.type == NNUE_T_F32) {
+#pragma unroll
+        for (int h = 0; h < HALF; h += 32) {
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+                    make_float4(acc[h + 4 * p], acc[h + 4 * p + 1], acc[h + 4 * p + 2], acc[h + 4 * p + 3]);
+            copy_rows_out(a.o, stg, 128, my_row, 0, col + h);
+        }
+    } else {
+        constexpr int kPass = HALF < 64 ? HALF : 64;
+#pragma unroll
+        for (int h = 0; h < HALF; h += kPass) {
+#pragma unroll
+            for (int p = 0; p < kPass / 8; ++p) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = pack_half(acc[h + 8 * p + 2 * j], acc[h + 8 * p + 2 * j + 1], a.o.type);
+                *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            copy_rows_out(a.o, stg, kPass * 2, my_row, 0, col + h);
+        }
+    }
+}
+
+template <int BN, int CTAS, bool SPLIT>
+__device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, uint64_t* done, uint64_t* taken, unsigned char* ring_ptr,
+                                               unsigned char* staging, int t0, int stride, int tiles, int rank, int ranks) {
+    constexpr bool PAIR = CTAS == 2;
+    constexpr int A = f8_accs(BN), HALF = BN / 2;  // HALF: columns of an output warp
+    const int warp = (threadIdx.x >> 5) - kF8OutWarp, lane = threadIdx.x & 31;
+    const int q = warp & 3, half = warp >> 2;  // the quarter of tensor memory's lanes, the half of the columns
+    const int r = (PAIR ? rank * kGroupRows : 0) + q * 32 + lane;
+    const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + half * HALF;
+    unsigned char* stg = staging + warp * kStagingBytes;
+    StageRing<A> at;
+    F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t0, rank, ranks);
+    F8ScaleAt sp = f8_scale_at(a, x, r, x.col0 + half * HALF);
+    F8Scales s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f8_load_scale(sp, x.c0 + i, s.x[i], s.w[i]);
+    for (int t = t0; t < tiles; t += stride) {
+        // the next tile is looked up while this one multiplies: two loads behind one another are longer than a stage
+        const F8Tile next = f8_tile<BN, CTAS, SPLIT>(a, t + stride < tiles ? t + stride : t, rank, ranks);
+        const int32_t my_row = r >= x.count ? -1 : a.dense ? x.first + r : __ldg(a.plan.order + x.first + r);
+        const int col = x.col0 + half * HALF;
+        float acc[HALF];
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
+#pragma unroll 1
+        for (int c = x.c0; c < x.c1; ++c) {
+            const float scale = s.x[0] * s.w[0];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                s.x[i] = s.x[i + 1];
+                s.w[i] = s.w[i + 1];
+            }
+            f8_load_scale(sp, c + 4, s.x[3], s.w[3]);
+            if (!mbar_wait_warp(done + at.stage, at.phase)) return false;
+            tc_fence_after();
+            uint32_t v[2][32];
+            tmem_ld32(from + at.stage * BN, v[0]);
+            tmem_wait_ld(v[0]);
+#pragma unroll
+            for (int h = 0; h < HALF; h += 32) {
+                uint32_t(&now)[32] = v[h / 32 & 1];
+                if (h + 32 < HALF) {  // the next 32 columns come in during these products
+                    tmem_ld32(from + at.stage * BN + h + 32, v[~(h / 32) & 1]);
+                } else {  // the accumulator goes back before the last products
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR) mbar_arrive_cluster(map_rank(taken + at.stage, 0));
+                        else mbar_arrive(taken + at.stage);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) fma2(acc[h + j], acc[h + j + 1], now[j], now[j + 1], scale);
+                if (h + 32 < HALF) tmem_wait_ld(v[~(h / 32) & 1]);
+            }
+            at.next();
+        }
+        if (SPLIT) {
+            // the last accumulator is complete, so nothing reads the ring any more: it takes the partial tile
+            float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * (BN + 4) + half * HALF;
+#pragma unroll
+            for (int j = 0; j < HALF; j += 4) *reinterpret_cast<float4*>(part + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+            break;
+        }
+        sp = f8_scale_at(a, next, r, next.col0 + half * HALF);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f8_load_scale(sp, next.c0 + i, s.x[i], s.w[i]);
+        if (__any_sync(kFullMask, my_row >= 0) && col < a.o.cols) f8_bring_out<HALF>(a, x, acc, stg, my_row, col);
+        x = next;
+    }
+    return true;
+}
+
+// Split sums: row r of the tile is finished by rank r mod ranks, partial sums in the order of the ranks.
+template <int BN>
+__device__ __forceinline__ void f8_join(const F8Args& a, const F8Tile& x, uint32_t ring, int rank, int ranks) {
+    const int mine = (x.count - rank + ranks - 1) / ranks;
+    for (int i = threadIdx.x - kF8OutWarp * 32; i < mine * (BN / 4); i += kF8Threads - kF8OutWarp * 32) {
+        const int r = rank + i / (BN / 4) * ranks, c = i % (BN / 4) * 4, col = x.col0 + c;
+        if (col >= a.o.cols) continue;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (x.live) {
+            const uint32_t addr = ring + (uint32_t)(r * (BN + 4) + c) * 4;
+            for (int s = 0; s < ranks; ++s) {
+                const float4 p = ld_cluster4(addr, (uint32_t)s);
+                v[0] += p.x;
+                v[1] += p.y;
+                v[2] += p.z;
+                v[3] += p.w;
+            }
+            if (a.bias) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < a.o.cols) v[j] += __ldg(a.bias + (int64_t)x.bucket * a.N + col + j);
+            }
+        }
+        const int64_t row = a.dense ? x.first + r : __ldg(a.plan.order + x.first + r), at = row * a.o.ld + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < a.o.cols) store_from_float(a.o.out, a.o.type, at + j, v[j]);
+    }
+}
+
 template <int BN, int CTAS, bool SPLIT>
 __global__ void __launch_bounds__(kF8Threads, 1)
     k_fp8_linear(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ F8Args a) {
     constexpr bool PAIR = CTAS == 2;
-    constexpr int S = f8_stages(BN, CTAS), A = f8_accs(BN), HALF = BN / 2;  // HALF: columns of an output warp
+    constexpr int S = f8_stages(BN, CTAS), A = f8_accs(BN);
     constexpr uint32_t kTmemCols = A * BN;
-    constexpr int kPartPitch = BN + 4;  // floats per row of a partial tile
     static_assert(!(PAIR && SPLIT), "no such variant");
     extern __shared__ unsigned char smem_raw[];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -200,125 +383,32 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
 
-    bool ok = true;
-    if (warp == 0) {
-        ok = f8_copy_role<BN, CTAS, SPLIT>(a, &map_x, &map_w, ring, full, empty, t0, stride, tiles, rank, ranks);
-    } else if (warp == 1) {
-        if (lane == 0 && !(PAIR && rank != 0))
-            ok = f8_issue_role<BN, CTAS, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
+    if (warp < kF8OutWarp) {
+        if (BN == 256) fewer_registers<kF8FewRegs>();
+        bool ok = true;
+        if (warp == 0) {
+            ok = f8_copy_role<BN, CTAS, SPLIT>(a, &map_x, &map_w, ring, full, empty, t0, stride, tiles, rank, ranks);
+        } else if (warp == 1) {
+            if (lane == 0 && !(PAIR && rank != 0))
+                ok = f8_issue_role<BN, CTAS, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
+        }
+        __syncwarp();
+        if (!ok && lane == 0) note_timeout(a.status);
+        if (SPLIT) {
+            cluster_sync();
+            cluster_sync();
+        }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;  // the quarter of tensor memory's lanes, the half of the columns
-        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + half * HALF;
-        unsigned char* stg = staging + (warp - 2) * kStagingBytes;
-        StageRing<A> at;
-        for (int t = t0; t < tiles && ok; t += stride) {
-            const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t, rank, ranks);
-            const int r = (PAIR ? rank * kGroupRows : 0) + q * 32 + lane;
-            const int32_t my_row = r >= x.count ? -1 : a.dense ? x.first + r : __ldg(a.plan.order + x.first + r);
-            const int col = x.col0 + half * HALF;
-            const float* sx = a.x_scale + (int64_t)max(my_row, 0) * a.C;
-            const float* sw = a.w_scale + ((int64_t)(x.live ? x.bucket : 0) * a.R + min(col / kF8K, a.R - 1)) * a.C;
-            float acc[HALF];
-#pragma unroll
-            for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
-            float s_next = x.c1 > x.c0 && my_row >= 0 ? __ldg(sx + x.c0) * __ldg(sw + x.c0) : 0.f;
-            for (int c = x.c0; c < x.c1; ++c) {
-                const float s = s_next;
-                if (c + 1 < x.c1 && my_row >= 0) s_next = __ldg(sx + c + 1) * __ldg(sw + c + 1);
-                ok = mbar_wait_warp(done + at.stage, at.phase);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int h = 0; h < HALF; h += 32) {
-                    uint32_t v[32];
-                    tmem_ld32(from + at.stage * BN + h, v);
-                    tmem_wait_ld();
-                    if (h + 32 == HALF) {  // the accumulator goes back before the last products
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (PAIR) mbar_arrive_cluster(map_rank(taken + at.stage, 0));
-                            else mbar_arrive(taken + at.stage);
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) fma2(acc[h + j], acc[h + j + 1], v[j], v[j + 1], s);
-                }
-                at.next();
-            }
-            if (!ok) break;
-            if (SPLIT) {
-                // the last accumulator is complete, so nothing reads the ring any more: it takes the partial tile
-                float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * kPartPitch + half * HALF;
-#pragma unroll
-                for (int j = 0; j < HALF; j += 4) *reinterpret_cast<float4*>(part + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-                break;
-            }
-            if (!__any_sync(kFullMask, my_row >= 0) || col >= a.o.cols) continue;
-            if (a.bias && x.live) {
-                const float* b = a.bias + (int64_t)x.bucket * a.N + col;
-#pragma unroll
-                for (int j = 0; j < HALF; ++j)
-                    if (col + j < a.o.cols) acc[j] += __ldg(b + j);
-            }
-            if (a.o.type == NNUE_T_F32) {
-#pragma unroll
-                for (int h = 0; h < HALF; h += 32) {
-#pragma unroll
-                    for (int p = 0; p < 8; ++p)
-                        *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
-                            make_float4(acc[h + 4 * p], acc[h + 4 * p + 1], acc[h + 4 * p + 2], acc[h + 4 * p + 3]);
-                    copy_rows_out(a.o, stg, 128, my_row, 0, col + h);
-                }
-            } else {
-                constexpr int kPass = HALF < 64 ? HALF : 64;
-#pragma unroll
-                for (int h = 0; h < HALF; h += kPass) {
-#pragma unroll
-                    for (int p = 0; p < kPass / 8; ++p) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) w[j] = pack_half(acc[h + 8 * p + 2 * j], acc[h + 8 * p + 2 * j + 1], a.o.type);
-                        *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    copy_rows_out(a.o, stg, kPass * 2, my_row, 0, col + h);
-                }
-            }
+        if (BN == 256) more_registers<kF8ManyRegs>();
+        const bool ok = f8_output_role<BN, CTAS, SPLIT>(a, tmem, done, taken, ring_ptr, staging, t0, stride, tiles, rank, ranks);
+        if (!ok && lane == 0) note_timeout(a.status);
+        if (SPLIT) {
+            __syncwarp();
+            cluster_sync();
+            f8_join<BN>(a, f8_tile<BN, CTAS, SPLIT>(a, t0, rank, ranks), ring, rank, ranks);
+            __syncwarp();
+            cluster_sync();  // nobody leaves while its shared memory is read
         }
-    }
-    __syncwarp();
-    if (!ok && lane == 0) note_timeout(a.status);
-
-    if (SPLIT) {
-        cluster_sync();
-        // row r of the tile is finished by rank r mod ranks: partial sums in the order of the ranks
-        const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t0, rank, ranks);
-        const int mine = (x.count - rank + ranks - 1) / ranks;
-        for (int i = tid; i < mine * (BN / 4); i += kF8Threads) {
-            const int r = rank + i / (BN / 4) * ranks, c = i % (BN / 4) * 4, col = x.col0 + c;
-            if (col >= a.o.cols) continue;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            if (x.live) {
-                const uint32_t addr = ring + (uint32_t)(r * kPartPitch + c) * 4;
-                for (int s = 0; s < ranks; ++s) {
-                    const float4 p = ld_cluster4(addr, (uint32_t)s);
-                    v[0] += p.x;
-                    v[1] += p.y;
-                    v[2] += p.z;
-                    v[3] += p.w;
-                }
-                if (a.bias) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < a.o.cols) v[j] += __ldg(a.bias + (int64_t)x.bucket * a.N + col + j);
-                }
-            }
-            const int64_t row = a.dense ? x.first + r : __ldg(a.plan.order + x.first + r), at = row * a.o.ld + col;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < a.o.cols) store_from_float(a.o.out, a.o.type, at + j, v[j]);
-        }
-        cluster_sync();  // nobody leaves while its shared memory is read
     }
     tc_fence_before();
     __syncthreads();
@@ -334,6 +424,9 @@ int f8_launch(const CUtensorMap& mx, const CUtensorMap& mw, const F8Args& a, int
     NNUE_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !opted[dev]) {
         NNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, f8_smem(BN, CTAS)));
+        cudaFuncAttributes attr;
+        NNUE_CUDA_TRY(cudaFuncGetAttributes(&attr, kernel));
+        NNUE_REQUIRE(BN != 256 || attr.numRegs >= kF8LaunchRegs, NNUE_ERR_UNSUPPORTED, "fp8 linear: built with %d registers per thread", attr.numRegs);
         if (dev >= 0 && dev < 64) opted[dev] = true;
     }
     const int64_t at_once = sm_count() / CTAS;
@@ -359,7 +452,7 @@ int f8_launch(const CUtensorMap& mx, const CUtensorMap& mw, const F8Args& a, int
 
 using namespace nnue;
 
-extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, const float* x_scale, const void* w, int64_t ldw,
+extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, const float* x_scale, int64_t scale_ld, const void* w, int64_t ldw,
                                    const float* w_scale, const float* bias, const void* plan, void* y, int32_t y_type, int64_t T,
                                    int64_t K, int64_t N, int32_t E, int32_t format, void* stream) {
     const char* what = "nnue_fp8_linear_fwd";
@@ -374,6 +467,8 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, con
     if (T == 0) return NNUE_OK;
     NNUE_REQUIRE(x && w && x_scale && w_scale && y, NNUE_ERR_ARG, "%s: null pointer", what);
     if (laid) ldx = (K + 15) / 16 * 16;
+    NNUE_REQUIRE(scale_ld == 0 || (!plan && scale_ld >= T) || (laid && scale_ld >= group_laid_rows(T, E)), NNUE_ERR_ARG,
+                 "%s: scales by place need rows laid out by bucket, or one matrix, and room for every row", what);
     NNUE_REQUIRE(ldx >= K && ldw >= K, NNUE_ERR_ARG, "%s: pitch below the row length", what);
     NNUE_REQUIRE(aligned16(x) && aligned16(w) && ldx % 16 == 0 && ldw % 16 == 0, NNUE_ERR_ALIGN,
                  "%s: rows of x and w must start at multiples of 16 bytes", what);
@@ -382,6 +477,7 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, con
     if (plan) a.plan = group_view(plan, T, E);
     a.o = rows_out(y, y_type, N);
     a.x_scale = x_scale;
+    a.scale_ld = scale_ld;
     a.w_scale = w_scale;
     a.bias = bias;
     a.T = (int32_t)T;

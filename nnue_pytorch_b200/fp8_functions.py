@@ -85,8 +85,8 @@ def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn
     q, ldq = _empty_q(T, K, format, dev)
     scale = torch.empty(T, (K + BLOCK - 1) // BLOCK, dtype=torch.float32, device=dev)
     with _on(dev), _span("fp8_rows", dev):
-        st = _lib.load().nnue_fp8_quantize_rows(_ptr(x), TYPES[x.dtype], ldx, _ptr(q), ldq, _ptr(scale), T, K, TYPES[format],
-                                                None, 0, _stream(dev))
+        st = _lib.load().nnue_fp8_quantize_rows(_ptr(x), TYPES[x.dtype], ldx, _ptr(q), ldq, _ptr(scale), 0, T, K,
+                                                TYPES[format], None, 0, _stream(dev))
     _lib.check(st, "nnue_fp8_quantize_rows")
     return Fp8Blocks(q, scale)
 
@@ -158,22 +158,30 @@ def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tenso
     with _on(dev), _span("linear_fp8", dev):
         s = _stream(dev)
         wr, ldw = _pitched(weight.q, format, lib, dev)
-        if not given and not laid:
-            x = quantize_fp8_rows(x, format)
-        if not given and laid:
+        C = (K + BLOCK - 1) // BLOCK
+        if not given and (laid or plan is None):  # scales by block: what the product's warps read together lies together
             xs, ldx = _source(x)
-            xr = torch.empty(lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E), dtype=torch.uint8, device=dev)
-            scale = torch.empty(T, (K + BLOCK - 1) // BLOCK, dtype=torch.float32, device=dev)
-            _lib.check(lib.nnue_fp8_quantize_rows(_ptr(xs), TYPES[xs.dtype], ldx, _ptr(xr), 0, _ptr(scale), T, K, TYPES[format],
-                                                  buffer, E, s), "nnue_fp8_quantize_rows")
+            if laid:
+                nbytes = lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E)
+                xr, pitch = torch.empty(nbytes, dtype=torch.uint8, device=dev), 0
+                scale_ld = nbytes // ((K + 15) // 16 * 16)
+            else:
+                xr, pitch = _empty_q(T, K, format, dev)
+                scale_ld = T
+            scale = torch.empty(C, scale_ld, dtype=torch.float32, device=dev)
+            _lib.check(lib.nnue_fp8_quantize_rows(_ptr(xs), TYPES[xs.dtype], ldx, _ptr(xr), pitch, _ptr(scale), scale_ld, T, K,
+                                                  TYPES[format], buffer if laid else None, E, s), "nnue_fp8_quantize_rows")
+            ldx = pitch
         else:
-            scale = x.scale
+            if not given:
+                x = quantize_fp8_rows(x, format)
+            scale, scale_ld = x.scale, 0
             xr, ldx = _pitched(x.q, format, lib, dev, whole=laid)
             if laid:  # pairs of bytes as 16-bit numbers, moved as they are
                 src, xr = xr, torch.empty(lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E), dtype=torch.uint8, device=dev)
                 _lib.check(lib.nnue_group_rows(_ptr(src), TYPES[torch.bfloat16], ldx // 2, buffer, _ptr(xr), TYPES[torch.bfloat16],
                                                None, T, (K + 15) // 16 * 8, E, s), "nnue_group_rows")
-        st = lib.nnue_fp8_linear_fwd(_ptr(xr), ldx, laid, _ptr(scale), _ptr(wr), ldw, _ptr(weight.scale), _ptr(bias), buffer,
+        st = lib.nnue_fp8_linear_fwd(_ptr(xr), ldx, laid, _ptr(scale), scale_ld, _ptr(wr), ldw, _ptr(weight.scale), _ptr(bias), buffer,
                                      _ptr(y), TYPES[out_dtype], T, K, N, E, TYPES[format], s)
     _lib.check(st, "nnue_fp8_linear_fwd")
     return y

@@ -70,16 +70,18 @@ def test_grouped_linear_arguments(lib):
 
 def test_fp8_arguments(lib):
     P = 1 << 20
-    rows = lambda **k: lib.nnue_fp8_quantize_rows(*({**dict(x=P, t=1, ldx=64, q=P, ldq=64, s=P, T=4, K=64, f=3, plan=None, E=0), **k}.values()), None)  # noqa: E731
+    rows = lambda **k: lib.nnue_fp8_quantize_rows(*({**dict(x=P, t=1, ldx=64, q=P, ldq=64, s=P, sl=0, T=4, K=64, f=3, plan=None, E=0), **k}.values()), None)  # noqa: E731
     assert rows(T=0) == 0 and rows(T=-1) == -1 and rows(K=0) == -1 and rows(ldx=63) == -1 and rows(ldq=63) == -1 and rows(ldq=129) == -1
     assert rows(plan=P) == -1 and rows(plan=P, E=1025) == -1 and rows(plan=P + 4, E=2) == -1 and rows(plan=P, E=2, ldq=0, T=0) == 0
     assert rows(t=3) == -4 and rows(f=1) == -4 and rows(x=None) == -1 and rows(s=None) == -1
+    assert rows(sl=3) == -1 and rows(sl=4, T=0) == 0 and rows(plan=P, E=2, sl=4) == -1
     tiles = lambda **k: lib.nnue_fp8_quantize_tiles(*({**dict(x=P, t=1, ldx=64, q=P, ldq=64, s=P, E=1, N=4, K=64, f=3), **k}.values()), None)  # noqa: E731
     assert tiles(E=0) == -1 and tiles(N=0) == 0 and tiles(f=0) == -4 and tiles(q=None) == -1
-    lin = lambda **k: lib.nnue_fp8_linear_fwd(*({**dict(x=P, ldx=64, laid=0, sx=P, w=P, ldw=64, sw=P, b=None, plan=P, y=P, yt=1, T=4, K=64, N=8, E=2, f=3), **k}.values()), None)  # noqa: E731
+    lin = lambda **k: lib.nnue_fp8_linear_fwd(*({**dict(x=P, ldx=64, laid=0, sx=P, sl=0, w=P, ldw=64, sw=P, b=None, plan=P, y=P, yt=1, T=4, K=64, N=8, E=2, f=3), **k}.values()), None)  # noqa: E731
     assert lin(T=0) == 0 and lin(plan=None) == -1 and lin(plan=None, E=1, T=0) == 0 and lin(plan=None, E=1, laid=1) == -1 and lin(f=1) == -4 and lin(yt=4) == -4
     assert lin(sx=None) == -1 and lin(sw=None) == -1 and lin(y=None) == -1 and lin(ldx=65) == -2 and lin(ldw=72) == -2
     assert lin(w=P + 8) == -2 and lin(y=P + 1) == -2 and lin(ldx=48) == -1 and lin(E=2000) == -4
+    assert lin(sl=8) == -1 and lin(sl=4, laid=1) == -1 and lin(sl=3, plan=None, E=1) == -1
 
 
 def test_python_refusals():
