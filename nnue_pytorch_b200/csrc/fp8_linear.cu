@@ -12,27 +12,31 @@
 // bucket (the quantiser leaves them so), in their own order where there is one matrix, or are gathered by TMA, four per
 // copy, where a bucket has few.
 #include "grouped_tc.cuh"
-
 namespace nnue {
 
 constexpr int kF8K = 128;
 constexpr int kF8ABytes = kGroupRows * 128;
-constexpr int kF8Threads = 384;  // copies, instructions, two warps without work, eight output warps
+constexpr int kF8Threads = 384;  // copies, instructions, scales, a warp without work, eight output warps
 constexpr int kF8OutWarp = 4;    // the first output warp
 // An output thread of the widest tile holds 128 sums and two reads of 32 columns: the first warpgroup gives registers up.
-constexpr int kF8FewRegs = 56, kF8ManyRegs = 224, kF8LaunchRegs = 168;
+constexpr int kF8FewRegs = 72, kF8ManyRegs = 216, kF8LaunchRegs = 168;
 static_assert(128 * kF8FewRegs + 256 * kF8ManyRegs <= kF8Threads * kF8LaunchRegs, "more registers than the launch brings");
 
 constexpr int f8_stage_bytes(int bn, int ctas) { return kF8ABytes + bn / ctas * 128; }
-constexpr int f8_stages(int bn, int ctas) { return f8_stage_bytes(bn, ctas) > 32768 ? 4 : f8_stage_bytes(bn, ctas) > 24576 ? 6 : 8; }
 constexpr int f8_accs(int bn) { return bn == 256 ? 2 : 4; }
-constexpr int f8_smem(int bn, int ctas) { return 1024 + f8_stages(bn, ctas) * f8_stage_bytes(bn, ctas) + 8 * kStagingBytes + 256; }
+constexpr int kF8Groups = 2;  // groups of scales of four stages each
+constexpr int kF8Slots = 4 * kF8Groups;
+constexpr int f8_slot_floats(int bn) { return kGroupRows * (bn == 256 ? 2 : 1); }
+constexpr int f8_rest(int bn) { return 1024 + 8 * kStagingBytes + kF8Slots * f8_slot_floats(bn) * 4 + 512; }  // alignment, staging, scales, barriers
+constexpr int f8_stages(int bn, int ctas) { return (232448 - f8_rest(bn)) / f8_stage_bytes(bn, ctas); }  // what 227 KB hold
+constexpr int f8_smem(int bn, int ctas) { return f8_rest(bn) + f8_stages(bn, ctas) * f8_stage_bytes(bn, ctas); }
 
 struct F8Args {
     GroupPlanView plan;
     RowsOut o;
     const float *x_scale, *w_scale, *bias;
     int64_t scale_ld;    // 0: x_scale [T, C] by rows of the batch; else [C, scale_ld] by the rows' places in x
+    int32_t scale_vec;   // the latter, four rows at a time
     int32_t T, E, N, K;
     int32_t C, R;        // blocks along K and along N
     int32_t col_tiles;
@@ -120,24 +124,28 @@ __device__ __forceinline__ bool f8_issue_role(const F8Args& a, uint32_t tmem, ui
     for (int t = t0; t < tiles && ok; t += stride) {
         const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t, rank, ranks);
         for (int c = x.c0; c < x.c1; ++c) {
-            ok = mbar_wait_timed(taken + acc.stage, acc.phase ^ 1u) && mbar_wait_timed(full + at.stage, at.phase);
+            ok = mbar_wait_warp(taken + acc.stage, acc.phase ^ 1u) && mbar_wait_warp(full + at.stage, at.phase);
             if (!ok) break;
             tc_fence_after();
             const uint32_t sa = ring + at.stage * f8_stage_bytes(BN, CTAS);
             const uint64_t da = umma_desc_sw128(sa, 16), db = umma_desc_sw128(sa + kF8ABytes, 16);
             const int steps = min(4, (a.K - c * kF8K + 31) >> 5);  // instructions of 32 inputs
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k < steps) umma_f8<PAIR>(tmem + acc.stage * BN, da + 2 * k, db + 2 * k, a.idesc, k != 0);
-            umma_commit_to<PAIR>(empty + at.stage);
-            umma_commit_to<PAIR>(done + acc.stage);
+                for (int k = 0; k < 4; ++k)
+                    if (k < steps) umma_f8<PAIR>(tmem + acc.stage * BN, da + 2 * k, db + 2 * k, a.idesc, k != 0);
+                umma_commit_to<PAIR>(empty + at.stage);
+                umma_commit_to<PAIR>(done + acc.stage);
+            }
+            __syncwarp();
             at.next();
             acc.next();
         }
     }
     if (!ok) {  // instructions in flight finish before the tensor memory is freed
-        umma_commit_to<PAIR>(drained);
-        mbar_wait_timed(drained, 0);
+        if (elect_one()) umma_commit_to<PAIR>(drained);
+        __syncwarp();
+        mbar_wait_warp(drained, 0);
     }
     return ok;
 }
@@ -152,36 +160,60 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
 }
 
-// Scales of four consecutive stages of one thread: its row's and its columns'.
-struct F8Scales {
-    float x[4], w[4];
-};
-struct F8ScaleAt {
-    const float *x, *w;
-    int64_t step;  // of x from one block to the next
-    int32_t end;
-};
-__device__ __forceinline__ F8ScaleAt f8_scale_at(const F8Args& a, const F8Tile& x, int r, int col) {
-    F8ScaleAt s;
-    const bool mine = r < x.count;
-    if (a.scale_ld) {
-        s.x = a.x_scale + (mine ? x.place + r : 0);
-        s.step = a.scale_ld;
-    } else {
-        const int row = !mine ? 0 : a.dense ? x.first + r : __ldg(a.plan.order + x.first + r);
-        s.x = a.x_scale + (int64_t)row * a.C;
-        s.step = 1;
+// One warp: sx * sw of every row and half of the columns, four stages at a time, into the ring that the output warps read.
+// (As loads of the output warps themselves they were waited for in every stage: their registers hold the sums.)
+template <int BN, int CTAS, bool SPLIT>
+__device__ __forceinline__ bool f8_scale_role(const F8Args& a, float* slots, uint64_t* sfull, uint64_t* sfree, int t0, int stride,
+                                              int tiles, int rank, int ranks) {
+    constexpr int kHalves = f8_slot_floats(BN) / kGroupRows;
+    const int lane = threadIdx.x & 31, r0 = 4 * lane + (CTAS == 2 ? rank * kGroupRows : 0);
+    StageRing<kF8Groups> at;
+    for (int t = t0; t < tiles; t += stride) {
+        const F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t, rank, ranks);
+        const int left = x.count - r0;  // rows of the lane's four that there are
+        const float* sx[4];
+        const int64_t step = a.scale_ld ? a.scale_ld : 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = j < left ? r0 + j : 0;
+            sx[j] = a.x_scale + (a.scale_ld ? x.place + r : (int64_t)(a.dense ? x.first + r : x.live ? __ldg(a.plan.order + x.first + r) : 0) * a.C);
+        }
+        const float* sw[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+            sw[h] = a.w_scale + ((int64_t)(x.live ? x.bucket : 0) * a.R + min(x.col0 / kF8K + h, a.R - 1)) * a.C;
+        for (int c4 = x.c0; c4 < x.c1; c4 += 4) {
+            float v[4][4], w[4][kHalves];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = min(c4 + i, x.c1 - 1);
+                if (a.scale_vec && left >= 4) {
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(sx[0] + c * step));
+                    v[i][0] = f.x;
+                    v[i][1] = f.y;
+                    v[i][2] = f.z;
+                    v[i][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i][j] = j < left ? __ldg(sx[j] + c * step) : 0.f;
+                }
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h) w[i][h] = __ldg(sw[h] + c);
+            }
+            if (!mbar_wait_warp(sfree + at.stage, at.phase ^ 1u)) return false;
+            float* to = slots + at.stage * 4 * f8_slot_floats(BN) + 4 * lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+                    *reinterpret_cast<float4*>(to + i * f8_slot_floats(BN) + h * kGroupRows) =
+                        make_float4(v[i][0] * w[i][h], v[i][1] * w[i][h], v[i][2] * w[i][h], v[i][3] * w[i][h]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfull + at.stage);
+            at.next();
+        }
     }
-    s.w = a.w_scale + ((int64_t)(x.live ? x.bucket : 0) * a.R + min(col / kF8K, a.R - 1)) * a.C;
-    s.end = mine ? x.c1 : 0;
-    return s;
-}
-__device__ __forceinline__ void f8_load_scale(const F8ScaleAt& s, int c, float& x, float& w) {
-    x = w = 0.f;
-    if (c < s.end) {
-        x = __ldg(s.x + c * s.step);
-        w = __ldg(s.w + c);
-    }
+    return true;
 }
 
 // An output warp's 32 rows and half of the columns, from registers to the output.
@@ -229,61 +261,75 @@ __device__ __forceinline__ void f8_bring_out(const F8Args& a, const F8Tile& x, f
 }
 
 template <int BN, int CTAS, bool SPLIT>
-__device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, uint64_t* done, uint64_t* taken, unsigned char* ring_ptr,
-                                               unsigned char* staging, int t0, int stride, int tiles, int rank, int ranks) {
+__device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, uint64_t* done, uint64_t* taken, const float* slots,
+                                               uint64_t* sfull, uint64_t* sfree, unsigned char* ring_ptr, unsigned char* staging,
+                                               int t0, int stride, int tiles, int rank, int ranks) {
     constexpr bool PAIR = CTAS == 2;
     constexpr int A = f8_accs(BN), HALF = BN / 2;  // HALF: columns of an output warp
     const int warp = (threadIdx.x >> 5) - kF8OutWarp, lane = threadIdx.x & 31;
     const int q = warp & 3, half = warp >> 2;  // the quarter of tensor memory's lanes, the half of the columns
     const int r = (PAIR ? rank * kGroupRows : 0) + q * 32 + lane;
     const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + half * HALF;
+    const float* my_scale = slots + (BN == 256 ? half * kGroupRows : 0) + q * 32 + lane;
     unsigned char* stg = staging + warp * kStagingBytes;
     StageRing<A> at;
+    StageRing<kF8Groups> sat;
     F8Tile x = f8_tile<BN, CTAS, SPLIT>(a, t0, rank, ranks);
-    F8ScaleAt sp = f8_scale_at(a, x, r, x.col0 + half * HALF);
-    F8Scales s;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f8_load_scale(sp, x.c0 + i, s.x[i], s.w[i]);
     for (int t = t0; t < tiles; t += stride) {
-        // the next tile is looked up while this one multiplies: two loads behind one another are longer than a stage
+        // the next tile is looked up while this one multiplies
         const F8Tile next = f8_tile<BN, CTAS, SPLIT>(a, t + stride < tiles ? t + stride : t, rank, ranks);
         const int32_t my_row = r >= x.count ? -1 : a.dense ? x.first + r : __ldg(a.plan.order + x.first + r);
         const int col = x.col0 + half * HALF;
         float acc[HALF];
 #pragma unroll
         for (int j = 0; j < HALF; ++j) acc[j] = 0.f;
-#pragma unroll 1
-        for (int c = x.c0; c < x.c1; ++c) {
-            const float scale = s.x[0] * s.w[0];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                s.x[i] = s.x[i + 1];
-                s.w[i] = s.w[i + 1];
-            }
-            f8_load_scale(sp, c + 4, s.x[3], s.w[3]);
+        // Two reads of 32 columns are under way at any time, the first two of the next stage during this one's last products.
+        constexpr int kReads = HALF / 32;
+        uint32_t v[2][32];
+        if (x.c0 < x.c1) {
             if (!mbar_wait_warp(done + at.stage, at.phase)) return false;
             tc_fence_after();
-            uint32_t v[2][32];
-            tmem_ld32(from + at.stage * BN, v[0]);
-            tmem_wait_ld(v[0]);
 #pragma unroll
-            for (int h = 0; h < HALF; h += 32) {
-                uint32_t(&now)[32] = v[h / 32 & 1];
-                if (h + 32 < HALF) {  // the next 32 columns come in during these products
-                    tmem_ld32(from + at.stage * BN + h + 32, v[~(h / 32) & 1]);
-                } else {  // the accumulator goes back before the last products
+            for (int h = 0; h < 2 && h < kReads; ++h) tmem_ld32(from + at.stage * BN + 32 * h, v[h]);
+        }
+#pragma unroll 1
+        for (int c = x.c0; c < x.c1; ++c) {
+            const int in_group = (c - x.c0) & 3;
+            if (in_group == 0 && !mbar_wait_warp(sfull + sat.stage, sat.phase)) return false;
+            const float scale = my_scale[(sat.stage * 4 + in_group) * f8_slot_floats(BN)];
+            const bool more = c + 1 < x.c1;
+            const int now = at.stage;
+            at.next();
+            tmem_wait_ld(v[0]);
+            if (kReads > 1) tmem_wait_ld(v[1]);
+#pragma unroll
+            for (int h = 0; h < kReads; ++h) {
+                if (h + 2 == kReads || kReads == 1) {  // all of it is in registers: the accumulator goes back
+                    if (h > 0) {
+                        tmem_wait_ld(v[0]);
+                        tmem_wait_ld(v[1]);
+                    }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        if (PAIR) mbar_arrive_cluster(map_rank(taken + at.stage, 0));
-                        else mbar_arrive(taken + at.stage);
+                        if (PAIR) mbar_arrive_cluster(map_rank(taken + now, 0));
+                        else mbar_arrive(taken + now);
+                        if (in_group == 3 || !more) mbar_arrive(sfree + sat.stage);
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) fma2(acc[h + j], acc[h + j + 1], now[j], now[j + 1], scale);
-                if (h + 32 < HALF) tmem_wait_ld(v[~(h / 32) & 1]);
+                for (int j = 0; j < 32; j += 2) fma2(acc[32 * h + j], acc[32 * h + j + 1], v[h & 1][j], v[h & 1][j + 1], scale);
+                if (h + 2 < kReads) {
+                    tmem_ld32(from + now * BN + 32 * (h + 2), v[h & 1]);
+                } else if (more) {
+                    if (h + 2 == kReads || kReads == 1) {
+                        if (!mbar_wait_warp(done + at.stage, at.phase)) return false;
+                        tc_fence_after();
+                    }
+                    tmem_ld32(from + at.stage * BN + 32 * (h & 1), v[h & 1]);
+                }
             }
-            at.next();
+            if (in_group == 3 || !more) sat.next();
         }
         if (SPLIT) {
             // the last accumulator is complete, so nothing reads the ring any more: it takes the partial tile
@@ -292,9 +338,6 @@ __device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, u
             for (int j = 0; j < HALF; j += 4) *reinterpret_cast<float4*>(part + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
             break;
         }
-        sp = f8_scale_at(a, next, r, next.col0 + half * HALF);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f8_load_scale(sp, next.c0 + i, s.x[i], s.w[i]);
         if (__any_sync(kFullMask, my_row >= 0) && col < a.o.cols) f8_bring_out<HALF>(a, x, acc, stg, my_row, col);
         x = next;
     }
@@ -342,11 +385,14 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
     unsigned char* staging = ring_ptr + S * f8_stage_bytes(BN, CTAS);
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * kStagingBytes);  // [S] a stage's copies are in (pair: the first CTA's)
+    float* slots = reinterpret_cast<float*>(staging + 8 * kStagingBytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(slots + kF8Slots * f8_slot_floats(BN));  // [S] a stage's copies are in (pair: the first CTA's)
     uint64_t* empty = full + S;                                                 // [S] a stage may be overwritten
     uint64_t* done = empty + S;                                                 // [A] an accumulator is complete
     uint64_t* taken = done + A;                                                 // [A] an accumulator has been read
-    uint64_t* drained = taken + A;                                              // [1]
+    uint64_t* sfull = taken + A;                                                // [kF8Groups] a group of scales is there
+    uint64_t* sfree = sfull + kF8Groups;                                        // [kF8Groups] and has been read
+    uint64_t* drained = sfree + kF8Groups;                                      // [1]
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -371,6 +417,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             mbar_init(done + s, 1);
             mbar_init(taken + s, 8 * CTAS);
         }
+        for (int s = 0; s < kF8Groups; ++s) {
+            mbar_init(sfull + s, 1);
+            mbar_init(sfree + s, 8);
+        }
         mbar_init(drained, 1);
         fence_barrier_init();
         prefetch_map(&map_x);
@@ -389,8 +439,10 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         if (warp == 0) {
             ok = f8_copy_role<BN, CTAS, SPLIT>(a, &map_x, &map_w, ring, full, empty, t0, stride, tiles, rank, ranks);
         } else if (warp == 1) {
-            if (lane == 0 && !(PAIR && rank != 0))
+            if (!(PAIR && rank != 0))
                 ok = f8_issue_role<BN, CTAS, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
+        } else if (warp == 2) {
+            ok = f8_scale_role<BN, CTAS, SPLIT>(a, slots, sfull, sfree, t0, stride, tiles, rank, ranks);
         }
         __syncwarp();
         if (!ok && lane == 0) note_timeout(a.status);
@@ -400,7 +452,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
     } else {
         if (BN == 256) more_registers<kF8ManyRegs>();
-        const bool ok = f8_output_role<BN, CTAS, SPLIT>(a, tmem, done, taken, ring_ptr, staging, t0, stride, tiles, rank, ranks);
+        const bool ok = f8_output_role<BN, CTAS, SPLIT>(a, tmem, done, taken, slots, sfull, sfree, ring_ptr, staging, t0, stride, tiles, rank, ranks);
         if (!ok && lane == 0) note_timeout(a.status);
         if (SPLIT) {
             __syncwarp();
@@ -448,6 +500,20 @@ int f8_launch(const CUtensorMap& mx, const CUtensorMap& mw, const F8Args& a, int
     return NNUE_OK;
 }
 
+// Pairs on 256 columns or CTAs on up to 128.  A round of the latter takes about 5/8 of a pair's round for half the work: at
+// 4099 x 2000 x 1500 two rounds of pairs, 1.4 full, came to 55 us and three of single CTAs, 2.7 full, to 50; at 16384 x 4096
+// x 2048 over 8 buckets eight rounds of pairs to 178 us, against 223 for pairs on 128 columns.
+static TileShape f8_shape(int64_t runs, int64_t T, int64_t N, int64_t chunks, bool pairs) {
+    const int64_t rows = (T + runs - 1) / runs, sms = sm_count();
+    auto rounds = [&](int64_t high, int64_t wide, int64_t at_once) {
+        return (runs * ((rows + high - 1) / high) * ((N + wide - 1) / wide) + at_once - 1) / at_once;
+    };
+    const TileShape narrow = tile_shape(runs, rows, N, chunks, 64, 128, false);
+    if (pairs && narrow.bn == 128 && rows > kGroupRows && rounds(kGroupPairRows, 256, sms / 2) * 8 <= rounds(kGroupRows, 128, sms) * 5)
+        return {256, 2, 1};
+    return narrow;
+}
+
 }  // namespace nnue
 
 using namespace nnue;
@@ -478,6 +544,7 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, con
     a.o = rows_out(y, y_type, N);
     a.x_scale = x_scale;
     a.scale_ld = scale_ld;
+    a.scale_vec = scale_ld > 0 && scale_ld % 4 == 0 && aligned16(x_scale);
     a.w_scale = w_scale;
     a.bias = bias;
     a.T = (int32_t)T;
@@ -492,8 +559,7 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, con
     NNUE_REQUIRE(a.status, NNUE_ERR_CUDA, "%s: no device status word", what);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("fp8_linear", s);
-    const int64_t runs = E < T ? E : T;
-    const TileShape shape = tile_shape(runs, (T + runs - 1) / runs, N, a.C, 64, 256, !a.gather);
+    const TileShape shape = f8_shape(E < T ? E : T, T, N, a.C, !a.gather);
     a.col_tiles = (int32_t)((N + shape.bn - 1) / shape.bn);
     a.idesc = umma_idesc(format == NNUE_T_E5M2 ? 1u : 0u, (uint32_t)(kGroupRows * shape.ctas), (uint32_t)shape.bn, 0, 0);
     CUtensorMap mx, mw;
@@ -512,6 +578,5 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, con
     if (shape.ctas == 2) return f8_launch<256, 2, false>(mx, mw, a, tiles, 1, s);
     const bool split = shape.ranks > 1;
     if (shape.bn == 64) return split ? f8_launch<64, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<64, 1, false>(mx, mw, a, tiles, 1, s);
-    if (shape.bn == 128) return split ? f8_launch<128, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<128, 1, false>(mx, mw, a, tiles, 1, s);
-    return split ? f8_launch<256, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<256, 1, false>(mx, mw, a, tiles, 1, s);
+    return split ? f8_launch<128, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<128, 1, false>(mx, mw, a, tiles, 1, s);
 }

@@ -216,7 +216,7 @@ __device__ __forceinline__ bool gl_copy_role(const GlArgs& a, const CUtensorMap*
     return ok;
 }
 
-// ---- one thread: the instructions -------------------------------------------------------------------------------------
+// ---- warp 1: the instructions -------------------------------------------------------------------------------------
 template <int MODE, int BN, int CTAS, bool SPLIT, bool LONG>
 __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, uint32_t ring, uint64_t* full, uint64_t* empty,
                                               uint64_t* done, uint64_t* taken, uint64_t* drained, int t0, int stride, int tiles,
@@ -231,31 +231,35 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
         const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
         for (int g = x.c0; g < x.c1 && ok; g += LONG ? kGlLong : x.c1 - x.c0) {  // one accumulator's chunks
             const int end = LONG ? min(x.c1, g + kGlLong) : x.c1;
-            ok = mbar_wait_timed(taken + acc.stage, acc.phase ^ 1u);
+            ok = mbar_wait_warp(taken + acc.stage, acc.phase ^ 1u);
             if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem + acc.stage * BN;
             for (int c = g; c < end; ++c) {
-                ok = mbar_wait_timed(full + at.stage, at.phase);
+                ok = mbar_wait_warp(full + at.stage, at.phase);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t sa = ring + at.stage * gl_stage_bytes(BN, CTAS);
                 const uint64_t da = umma_desc_sw128(sa, kGlBoxBytes), db = umma_desc_sw128(sa + kGlABytes, kGlBoxBytes);
                 const int steps = gl_steps<MODE>(a, x, c);
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (k < steps) umma_f16<PAIR>(d, da + k * kAStep, db + k * kBStep, a.idesc, c != g || k != 0);
-                umma_commit_to<PAIR>(empty + at.stage);
+                    for (int k = 0; k < 4; ++k)
+                        if (k < steps) umma_f16<PAIR>(d, da + k * kAStep, db + k * kBStep, a.idesc, c != g || k != 0);
+                    umma_commit_to<PAIR>(empty + at.stage);
+                    if (c + 1 == end) umma_commit_to<PAIR>(done + acc.stage);
+                }
+                __syncwarp();
                 at.next();
             }
             if (!ok) break;
-            umma_commit_to<PAIR>(done + acc.stage);
             acc.next();
         }
     }
     if (!ok) {  // instructions in flight finish before the tensor memory is freed
-        umma_commit_to<PAIR>(drained);
-        mbar_wait_timed(drained, 0);
+        if (elect_one()) umma_commit_to<PAIR>(drained);
+        __syncwarp();
+        mbar_wait_warp(drained, 0);
     }
     return ok;
 }
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
     if (warp == 0) {
         ok = gl_copy_role<MODE, BN, CTAS, SPLIT>(a, &map_a, &map_b, ring, full, empty, t0, stride, tiles, rank, ranks);
     } else if (warp == 1) {
-        if (lane == 0 && !(PAIR && rank != 0))
+        if (!(PAIR && rank != 0))
             ok = gl_issue_role<MODE, BN, CTAS, SPLIT, LONG>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
     } else {
         const int q = warp & 3;  // the quarter of tensor memory's lanes that this warp may read

@@ -41,11 +41,22 @@ __device__ __forceinline__ bool mbar_wait_timed(uint64_t* bar, unsigned parity) 
     } while (clock64() - start < kWaitCycles);
     return false;
 }
-// The same for a whole warp, one lane asking.
+// The same for a whole warp: all lanes ask together, one instruction.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, unsigned parity) {
-    bool ok = true;
-    if ((threadIdx.x & 31) == 0) ok = mbar_wait_timed(bar, parity);
-    return __shfl_sync(kFullMask, (int)ok, 0) != 0;
+    const bool ok = __all_sync(kFullMask, mbar_wait_timed(bar, parity));
+    return ok;
+}
+
+// True in one lane of a converged warp.  Issued from such a branch of a warp that runs its loop together, tensor-core
+// instructions take their operands from uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -228,7 +239,7 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 // On another CTA's barrier, for reads of tensor memory that tc_fence_before has closed.  (A release of cluster scope waits
 // for all of the warp's memory traffic: 8-bit product of 16384 x 4096 x 2048, one arrival per stage and warp, 330 us; so 178.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ float4 ld_cluster4(uint32_t smem_addr, uint32_t rank) {
     float4 v;

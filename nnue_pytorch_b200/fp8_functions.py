@@ -164,10 +164,10 @@ def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tenso
             if laid:
                 nbytes = lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E)
                 xr, pitch = torch.empty(nbytes, dtype=torch.uint8, device=dev), 0
-                scale_ld = nbytes // ((K + 15) // 16 * 16)
+                scale_ld = (nbytes // ((K + 15) // 16 * 16) + 3) // 4 * 4
             else:
                 xr, pitch = _empty_q(T, K, format, dev)
-                scale_ld = T
+                scale_ld = (T + 3) // 4 * 4
             scale = torch.empty(C, scale_ld, dtype=torch.float32, device=dev)
             _lib.check(lib.nnue_fp8_quantize_rows(_ptr(xs), TYPES[xs.dtype], ldx, _ptr(xr), pitch, _ptr(scale), scale_ld, T, K,
                                                   TYPES[format], buffer if laid else None, E, s), "nnue_fp8_quantize_rows")
