@@ -5,16 +5,22 @@
 // the second term is a histogram of the rows before its slice plus the lanes below it that hold the same bucket
 // (one match instruction).  Work: ids read twice, order written once; bound by latency up to about a million rows.
 //
-// Batches of at most kSingleRows rows take ONE launch of one block (1024 threads, a counter per warp and bucket in shared
-// memory).  Longer ones take three: counters per block of rows, their scan, the fill; the launches cost about 2.5 us each,
-// which one block needs for some ten thousand rows.
+// Three forms, all with a counter per warp and bucket in shared memory, blocks of 1024 threads:
+//   up to   2048 rows  one block                                                          (2048 rows, 8 buckets: 10 us)
+//   up to  65536 rows  one cluster of eight blocks, which read one another's counters     (16384 rows: 12 us; one block 20)
+//   beyond             counters per block of 4096 rows, their scan, the fill: three launches, about 20 us of latency together
+//                      (65536 rows of 64 buckets: 24 us either way; 262143 of 256: 34, the cluster 64)
 #include "grouped.cuh"
+#include "tc.cuh"
 
 namespace nnue {
 
 constexpr int kGpThreads = 1024;
 constexpr int kGpWarps = kGpThreads / 32;
-constexpr int64_t kSingleRows = 16384;
+constexpr int kAhead = 4;  // ids per lane in flight
+constexpr int64_t kSingleRows = 2048;
+constexpr int64_t kClusterRows = 65536;
+constexpr int kClusterSize = 8;
 constexpr int kBlockRows = 4096;  // rows per block of the long form
 
 // bin of a row: its bucket, or E for -1 (padding row) and, with a note in the status word, for an id out of range
@@ -35,7 +41,14 @@ __device__ __forceinline__ void group_histogram(const Id* bucket, int64_t lo, in
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t per = (hi - lo + kGpWarps * 32 - 1) / (kGpWarps * 32) * 32;
     const int64_t a = lo + warp * per, b = min(hi, a + per);
-    for (int64_t p = a + lane; p < b; p += 32) atomicAdd(hist + warp * bins + group_bin(bucket, p, bins - 1, status), 1);
+    for (int64_t p0 = a + lane; p0 < b; p0 += 32 * kAhead) {
+        int bin[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) bin[u] = p0 + 32 * u < b ? group_bin(bucket, p0 + 32 * u, bins - 1, status) : -1;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (bin[u] >= 0) atomicAdd(hist + warp * bins + bin[u], 1);
+    }
     __syncthreads();
 }
 
@@ -59,20 +72,28 @@ __device__ __forceinline__ void group_fill(const Id* bucket, int64_t lo, int64_t
     const int64_t per = (hi - lo + kGpWarps * 32 - 1) / (kGpWarps * 32) * 32;
     const int64_t a = lo + warp * per, b = min(hi, a + per);
     int32_t* mine = hist + warp * bins;
-    for (int64_t p0 = a; p0 < b; p0 += 32) {
-        const int64_t p = p0 + lane;
-        const bool live = p < b;
-        const int bin = live ? group_bin(bucket, p, bins - 1, nullptr) : -1;
-        const unsigned same = __match_any_sync(kFullMask, bin);
-        const int rank = __popc(same & ((1u << lane) - 1u));
-        int at = 0;
-        if (live) at = mine[bin];
-        __syncwarp();
-        if (live) {
-            order[base[bin] + at + rank] = (int32_t)p;
-            if (rank == 0) mine[bin] = at + __popc(same);
+    for (int64_t p0 = a; p0 < b; p0 += 32 * kAhead) {
+        int bins_of[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t p = p0 + 32 * u + lane;
+            bins_of[u] = p < b ? group_bin(bucket, p, bins - 1, nullptr) : -1;
         }
-        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (p0 + 32 * u >= b) break;
+            const int bin = bins_of[u];
+            const unsigned same = __match_any_sync(kFullMask, bin);
+            const int rank = __popc(same & ((1u << lane) - 1u));
+            int at = 0;
+            if (bin >= 0) at = mine[bin];
+            __syncwarp();
+            if (bin >= 0) {
+                order[base[bin] + at + rank] = (int32_t)(p0 + 32 * u + lane);
+                if (rank == 0) mine[bin] = at + __popc(same);
+            }
+            __syncwarp();
+        }
     }
 }
 
@@ -101,9 +122,10 @@ __device__ __forceinline__ int4 block_scan4(int4 v, int4* s_warp, int4* total) {
     return make_int4(before.x + inc.x - v.x, before.y + inc.y - v.y, before.z + inc.z - v.z, before.w + inc.w - v.w);
 }
 
-// Totals of the bins (s_total) to the plan's offsets, places and tile lists.  s_at[bin] = first place in the order, first
+// Totals of the bins (s_total) to the plan's offsets, places and tile lists, shared out over `ranks` CTAs.  s_at[bin] = first place in the order, first
 // tile, first pair, first place among rows laid out by bucket.
-__device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_total, int4* s_at, int4* s_warp, int32_t* plan) {
+__device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_total, int4* s_at, int4* s_warp, int32_t* plan,
+                                            int rank = 0, int ranks = 1) {
     const int bins = E + 1;
     int4 carry = make_int4(0, 0, 0, 0);
     for (int b0 = 0; b0 < bins; b0 += kGpThreads) {
@@ -115,23 +137,27 @@ __device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_t
         const int4 at = add4(carry, block_scan4(mine, s_warp, &total));
         if (b < bins) {
             s_at[b] = at;
-            plan[group_offsets_at() + b] = at.x;
-            plan[group_places_at(T, E) + b] = at.w;
-            plan[group_first_at(T, E) + b] = at.y;
+            if (rank == 0) {
+                plan[group_offsets_at() + b] = at.x;
+                plan[group_places_at(T, E) + b] = at.w;
+                plan[group_first_at(T, E) + b] = at.y;
+            }
         }
         carry = add4(carry, total);
     }
     if (threadIdx.x == 0) {
         s_at[bins] = carry;
-        plan[0] = carry.y;
-        plan[1] = carry.z;
-        plan[group_offsets_at() + bins] = (int32_t)T;
+        if (rank == 0) {
+            plan[0] = carry.y;
+            plan[1] = carry.z;
+            plan[group_offsets_at() + bins] = (int32_t)T;
+        }
     }
     __syncthreads();
     for (int pairs = 0; pairs < 2; ++pairs) {
         int4* tiles = reinterpret_cast<int4*>(plan + (pairs ? group_pairs_at(T, E) : group_tiles_at(T, E)));
         const int rows = pairs ? kGroupPairRows : kGroupRows;
-        for (int t = threadIdx.x; t < (pairs ? carry.z : carry.y); t += kGpThreads) {
+        for (int t = rank * kGpThreads + threadIdx.x; t < (pairs ? carry.z : carry.y); t += ranks * kGpThreads) {
             int lo = 0, hi = bins - 1;  // the last bin whose first tile is not behind t; empty bins share a first tile
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -145,9 +171,10 @@ __device__ __forceinline__ void group_tiles(int64_t T, int E, const int32_t* s_t
     }
 }
 
-// shared memory: s_at [bins + 1] int4, counters per warp [bins][kGpWarps] (not in the scan), totals [bins]
+// shared memory: s_at [bins + 1] int4, counters per warp [bins][kGpWarps] (not in the scan), and three
+// arrays [bins]
 constexpr size_t group_smem_bytes(int bins, bool counters) {
-    return sizeof(int4) * (bins + 1) + sizeof(int32_t) * ((counters ? (size_t)bins * kGpWarps : 0) + bins);
+    return sizeof(int4) * (bins + 1) + sizeof(int32_t) * ((counters ? (size_t)bins * kGpWarps : 0) + 3 * (size_t)bins);
 }
 
 template <typename Id>
@@ -166,6 +193,42 @@ __global__ void __launch_bounds__(kGpThreads)
     for (int b = threadIdx.x; b < bins; b += kGpThreads) s_total[b] = s_at[b].x;  // from here on: first places
     __syncthreads();
     group_fill(bucket, 0, T, bins, s_hist, s_total, plan + group_order_at(E));
+}
+
+// One cluster: every CTA a run of the rows, the runs' counters read from one another's shared memory.
+template <typename Id>
+__global__ void __launch_bounds__(kGpThreads)
+    k_group_cluster(const Id* __restrict__ bucket, int64_t T, int E, int32_t* __restrict__ plan, unsigned long long* status) {
+    extern __shared__ int4 s_at[];
+    const int bins = E + 1, rank = (int)cluster_rank();
+    int32_t* s_hist = reinterpret_cast<int32_t*>(s_at + bins + 1);
+    int32_t* s_total = s_hist + bins * kGpWarps;
+    int32_t* s_own = s_total + bins;   // this CTA's counters
+    int32_t* s_base = s_own + bins;    // rows of the bin in the CTAs before; from there on first places
+    __shared__ int4 s_warp[kGpWarps];
+    const int64_t per = (T + kClusterSize * 32 - 1) / (kClusterSize * 32) * 32;
+    const int64_t lo = min(T, rank * per), hi = min(T, lo + per);
+    group_histogram(bucket, lo, hi, bins, s_hist, status);
+    for (int b = threadIdx.x; b < bins; b += kGpThreads) s_own[b] = group_scan_warps(s_hist, bins, b);
+    cluster_sync();
+    for (int b = threadIdx.x; b < bins; b += kGpThreads) {
+        int v[kClusterSize], total = 0, before = 0;
+#pragma unroll
+        for (int r = 0; r < kClusterSize; ++r) v[r] = ld_cluster_int(s_own + b, (uint32_t)r);
+#pragma unroll
+        for (int r = 0; r < kClusterSize; ++r) {
+            total += v[r];
+            if (r < rank) before += v[r];
+        }
+        s_total[b] = total;
+        s_base[b] = before;
+    }
+    __syncthreads();
+    group_tiles(T, E, s_total, s_at, s_warp, plan, rank, kClusterSize);
+    for (int b = threadIdx.x; b < bins; b += kGpThreads) s_base[b] += s_at[b].x;
+    __syncthreads();
+    group_fill(bucket, lo, hi, bins, s_hist, s_base, plan + group_order_at(E));
+    cluster_sync();  // nobody leaves while its counters are read
 }
 
 // long form, 1: counts[bin][block]
@@ -225,7 +288,7 @@ __global__ void __launch_bounds__(kGpThreads)
     group_fill(bucket, lo, hi, bins, s_hist, s_base, plan + group_order_at(E));
 }
 
-inline int64_t group_blocks(int64_t T) { return T <= kSingleRows ? 0 : (T + kBlockRows - 1) / kBlockRows; }
+inline int64_t group_blocks(int64_t T) { return T <= kClusterRows ? 0 : (T + kBlockRows - 1) / kBlockRows; }
 
 template <typename Id>
 int launch_plan(const Id* bucket, int64_t T, int32_t E, int32_t* plan, unsigned long long* status, cudaStream_t s) {
@@ -237,12 +300,27 @@ int launch_plan(const Id* bucket, int64_t T, int32_t E, int32_t* plan, unsigned 
     if (dev < 0 || dev >= 64 || !opted[dev]) {
         const int most = (int)group_smem_bytes(kMaxGroups + 1, true);
         NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_single<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+        NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_cluster<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_count<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         NNUE_CUDA_TRY(cudaFuncSetAttribute(k_group_fill<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
         if (dev >= 0 && dev < 64) opted[dev] = true;
     }
     const int64_t blocks = group_blocks(T);
-    if (blocks == 0) {
+    if (blocks == 0 && T > kSingleRows) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(kClusterSize);
+        cfg.blockDim = dim3(kGpThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = s;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kClusterSize;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        NNUE_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_group_cluster<Id>, bucket, T, (int)E, plan, status));
+        note_launches(1);
+    } else if (blocks == 0) {
         k_group_single<Id><<<1, kGpThreads, smem, s>>>(bucket, T, E, plan, status);
         note_launches(1);
     } else {

@@ -241,6 +241,11 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ int ld_cluster_int(const int* p, uint32_t rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(map_rank(p, rank)) : "memory");
+    return v;
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t smem_addr, uint32_t rank) {
     float4 v;
     asm volatile(

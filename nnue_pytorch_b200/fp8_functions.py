@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._launch import _ptr, _require_cuda, _span, _stream
+from ._launch import _outside_graphs, _ptr, _require_cuda, _span, _stream
 from .grouped_linear_functions import GATHERED_ROWS, TYPES, GroupPlan, _on, _pitched
 
 FORMATS = (torch.float8_e4m3fn, torch.float8_e5m2)
@@ -75,7 +75,7 @@ def _empty_q(rows: int, K: int, format: torch.dtype, dev) -> tuple[torch.Tensor,
     return (q if pitch == K else q[:, :K]), pitch
 
 
-@torch.compiler.disable
+@_outside_graphs
 def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
     """x [T, K] (fp32, bf16 or fp16) in 8 bits, one scale per 128 consecutive numbers of a row."""
     dev = _require_cuda(x)
@@ -91,7 +91,7 @@ def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn
     return Fp8Blocks(q, scale)
 
 
-@torch.compiler.disable
+@_outside_graphs
 def quantize_fp8_tiles(weight: torch.Tensor, count: int = 1, format: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
     """weight [count * N, K] (fp32, bf16 or fp16; `count` matrices below one another) in 8 bits, one scale per tile of
     128 x 128 of each matrix."""
@@ -112,7 +112,7 @@ def quantize_fp8_tiles(weight: torch.Tensor, count: int = 1, format: torch.dtype
     return Fp8Blocks(q, scale)
 
 
-@torch.compiler.disable
+@_outside_graphs
 def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tensor | None = None,
                plan: GroupPlan | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y[p] = weight[b(p)] x[p] + bias[b(p)] on 8-bit operands, fp32 sums; zeros for rows of no bucket.
@@ -159,22 +159,20 @@ def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tenso
         s = _stream(dev)
         wr, ldw = _pitched(weight.q, format, lib, dev)
         C = (K + BLOCK - 1) // BLOCK
-        if not given and (laid or plan is None):  # scales by block: what the product's warps read together lies together
+        if not given:
             xs, ldx = _source(x)
             if laid:
                 nbytes = lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E)
-                xr, pitch = torch.empty(nbytes, dtype=torch.uint8, device=dev), 0
-                scale_ld = (nbytes // ((K + 15) // 16 * 16) + 3) // 4 * 4
+                xr, pitch, places = torch.empty(nbytes, dtype=torch.uint8, device=dev), 0, nbytes // ((K + 15) // 16 * 16)
             else:
-                xr, pitch = _empty_q(T, K, format, dev)
-                scale_ld = (T + 3) // 4 * 4
-            scale = torch.empty(C, scale_ld, dtype=torch.float32, device=dev)
+                (xr, pitch), places = _empty_q(T, K, format, dev), T
+            # scales by block, four rows at a time, where the product's rows are neighbours; by row where it gathers them
+            scale_ld = (places + 3) // 4 * 4 if laid or plan is None else 0
+            scale = torch.empty(C * (scale_ld or T), dtype=torch.float32, device=dev)
             _lib.check(lib.nnue_fp8_quantize_rows(_ptr(xs), TYPES[xs.dtype], ldx, _ptr(xr), pitch, _ptr(scale), scale_ld, T, K,
                                                   TYPES[format], buffer if laid else None, E, s), "nnue_fp8_quantize_rows")
             ldx = pitch
         else:
-            if not given:
-                x = quantize_fp8_rows(x, format)
             scale, scale_ld = x.scale, 0
             xr, ldx = _pitched(x.q, format, lib, dev, whole=laid)
             if laid:  # pairs of bytes as 16-bit numbers, moved as they are

@@ -19,7 +19,7 @@ from torch import autograd
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._launch import _NO_SPAN, _ptr, _require_cuda, _span, _stream
+from ._launch import _NO_SPAN, _outside_graphs, _ptr, _require_cuda, _span, _stream
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.float8_e5m2: 4}
 HALF = (torch.bfloat16, torch.float16)
@@ -45,7 +45,7 @@ class GroupPlan:
 
     __slots__ = ("rows", "count", "device", "buffer")
 
-    @torch.compiler.disable
+    @_outside_graphs
     def __init__(self, bucket: torch.Tensor, count: int):
         dev = _require_cuda(bucket)
         assert bucket.dtype in (torch.int64, torch.int32), "bucket ids are int64 or int32"
@@ -118,43 +118,50 @@ def _laid_out(t: torch.Tensor, dtype: torch.dtype, plan_buffer, E: int, lib, dev
 GATHERED_ROWS = 16
 
 
+def _forward(x, weight, bias, plan, out_dtype, keep_rows):
+    """y, x as the product read it, the weights as it read them and their pitch.  `keep_rows`: x is laid out by bucket whatever
+    its length, as the weight gradient reads it."""
+    dev = _require_cuda(x, weight) if bias is None else _require_cuda(x, weight, bias)
+    dtype = x.dtype
+    assert dtype in HALF, "rows are bf16 or fp16"
+    assert weight.dtype in (dtype, torch.float32), "weights have the rows' type or are fp32"
+    out_dtype = out_dtype or dtype
+    assert out_dtype in (dtype, torch.float32), "the output has the rows' type or is fp32"
+    assert x.dim() == 2 and weight.dim() in (2, 3)
+    plan.check(x)
+    E = plan.count
+    w2 = weight.detach().flatten(0, 1) if weight.dim() == 3 else weight.detach()
+    T, K = x.shape
+    N = w2.shape[0] // E
+    assert K >= 1 and N >= 1 and w2.shape == (E * N, K) and (weight.dim() == 2 or weight.shape[0] == E), \
+        f"weight {tuple(weight.shape)} does not hold {E} layers of {K} inputs"
+    if bias is not None:
+        assert bias.dtype in (dtype, torch.float32) and bias.numel() == E * N
+        bias = bias.detach().contiguous()
+    lib = _lib.load()
+    y = torch.empty(T, N, dtype=out_dtype, device=dev)
+    laid = keep_rows or T > GATHERED_ROWS * E
+    with _on(dev), _span("grouped_linear_fwd", dev):
+        s = _stream(dev)
+        if laid:
+            xr, ldx = _laid_out(x.detach(), dtype, plan.buffer, E, lib, dev)[0], 0
+        else:
+            xr, ldx = _pitched(x.detach(), dtype, lib, dev)
+        wr, ldw = _pitched(w2, dtype, lib, dev)
+        st = lib.nnue_grouped_linear_fwd(
+            _ptr(xr), ldx, laid, _ptr(wr), ldw, _ptr(bias), 0 if bias is None else TYPES[bias.dtype], _ptr(plan.buffer), _ptr(y),
+            TYPES[out_dtype], T, K, N, E, TYPES[dtype], s)
+    _lib.check(st, "nnue_grouped_linear_fwd")
+    return y, xr, wr, ldw
+
+
 class GroupedLinearFunction(autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, plan, out_dtype=None):
-        dev = _require_cuda(x, weight) if bias is None else _require_cuda(x, weight, bias)
-        dtype = x.dtype
-        assert dtype in HALF, "rows are bf16 or fp16"
-        assert weight.dtype in (dtype, torch.float32), "weights have the rows' type or are fp32"
-        out_dtype = out_dtype or dtype
-        assert out_dtype in (dtype, torch.float32), "the output has the rows' type or is fp32"
-        assert x.dim() == 2 and weight.dim() in (2, 3)
-        plan.check(x)
-        E = plan.count
-        w2 = weight.detach().flatten(0, 1) if weight.dim() == 3 else weight.detach()
-        T, K = x.shape
-        N = w2.shape[0] // E
-        assert K >= 1 and N >= 1 and w2.shape == (E * N, K) and (weight.dim() == 2 or weight.shape[0] == E), \
-            f"weight {tuple(weight.shape)} does not hold {E} layers of {K} inputs"
-        if bias is not None:
-            assert bias.dtype in (dtype, torch.float32) and bias.numel() == E * N
-        lib = _lib.load()
-        y = torch.empty(T, N, dtype=out_dtype, device=dev)
-        # the weight gradient reads the rows laid out by bucket, and so does the forward unless they are few
-        laid = ctx.needs_input_grad[1] or T > GATHERED_ROWS * E
-        with _on(dev), _span("grouped_linear_fwd", dev):
-            if laid:
-                xr, ldx = _laid_out(x.detach(), dtype, plan.buffer, E, lib, dev)[0], 0
-            else:
-                xr, ldx = _pitched(x.detach(), dtype, lib, dev)
-            wr, ldw = _pitched(w2, dtype, lib, dev)
-            b = None if bias is None else bias.detach().contiguous()
-            st = lib.nnue_grouped_linear_fwd(
-                _ptr(xr), ldx, laid, _ptr(wr), ldw, _ptr(b), 0 if b is None else TYPES[b.dtype], _ptr(plan.buffer), _ptr(y),
-                TYPES[out_dtype], T, K, N, E, TYPES[dtype], _stream(dev))
-        _lib.check(st, "nnue_grouped_linear_fwd")
+        y, xr, wr, ldw = _forward(x, weight, bias, plan, out_dtype, ctx.needs_input_grad[1])
         ctx.save_for_backward(xr if ctx.needs_input_grad[1] else None, wr if ctx.needs_input_grad[0] else None, plan.buffer)
-        ctx.dims = (T, K, N, E, ldw)
-        ctx.dtype, ctx.w_like, ctx.b_like = dtype, (weight.dtype, weight.shape), None if bias is None else (bias.dtype, bias.shape)
+        ctx.dims = (*x.shape, y.shape[1], plan.count, ldw)
+        ctx.dtype, ctx.w_like, ctx.b_like = x.dtype, (weight.dtype, weight.shape), None if bias is None else (bias.dtype, bias.shape)
         return y
 
     @staticmethod
@@ -191,7 +198,7 @@ class GroupedLinearFunction(autograd.Function):
         return dx, dw, db, None, None
 
 
-@torch.compiler.disable  # ctypes launches: runs eagerly inside a compiled model
+@_outside_graphs  # ctypes launches: runs eagerly inside a compiled model
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, plan: GroupPlan,
                    out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """y[p] = weight[b(p)] x[p] + bias[b(p)], zeros for rows of no bucket.
@@ -202,4 +209,6 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     out_dtype  x's type (default) or float32
 
     Gradients: those of the formula, with dy rounded to x's type where it is fp32; each in its tensor's own type."""
-    return GroupedLinearFunction.apply(x, weight, bias, plan, out_dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return GroupedLinearFunction.apply(x, weight, bias, plan, out_dtype)
+    return _forward(x, weight, bias, plan, out_dtype, False)[0]
