@@ -52,40 +52,45 @@ constexpr int kLaneNumbers = 16;                                 // consecutive 
 constexpr int kWarpNumbers = 32 * kLaneNumbers;                  // four blocks of a row
 constexpr int kBlockLanes = kFp8Block / kLaneNumbers;            // 8
 
-// v[i] = p[at + i], zeros from i = left on
-__device__ __forceinline__ void load_sixteen(const void* p, int type, int64_t at, int left, bool vec, float (&v)[kLaneNumbers]) {
+// ROWS times sixteen numbers, v[u][i] = p[at[u] + i], zeros from i = left on and for u from n on.  All loads before any use.
+template <int TYPE, int ROWS>
+__device__ __forceinline__ void load_sixteen(const void* p, const int64_t (&at)[ROWS], int n, int left, bool vec,
+                                             float (&v)[ROWS][kLaneNumbers]) {
     if (vec && left >= kLaneNumbers) {
-        if (type == NNUE_T_F32) {
+        constexpr int kPieces = TYPE == NNUE_T_F32 ? 4 : 2;  // of 16 bytes
+        uint4 raw[ROWS][kPieces];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 f = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at) + i);
-                v[4 * i] = f.x;
-                v[4 * i + 1] = f.y;
-                v[4 * i + 2] = f.z;
-                v[4 * i + 3] = f.w;
+        for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                raw[u][i] = make_uint4(0, 0, 0, 0);
+                if (u < n) raw[u][i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at[u] * (TYPE == NNUE_T_F32 ? 4 : 2)) + i);
             }
-        } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at) + i);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t w[4] = {raw[u][i].x, raw[u][i].y, raw[u][i].z, raw[u][i].w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (type == NNUE_T_BF16) {
-                        v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-                        v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                    if (TYPE == NNUE_T_F32) {
+                        v[u][4 * i + j] = __uint_as_float(w[j]);
+                    } else if (TYPE == NNUE_T_BF16) {
+                        v[u][(8 * i + 2 * j) & 15] = __uint_as_float(w[j] << 16);
+                        v[u][(8 * i + 2 * j + 1) & 15] = __uint_as_float(w[j] & 0xffff0000u);
                     } else {
                         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-                        v[8 * i + 2 * j] = f.x;
-                        v[8 * i + 2 * j + 1] = f.y;
+                        v[u][(8 * i + 2 * j) & 15] = f.x;
+                        v[u][(8 * i + 2 * j + 1) & 15] = f.y;
                     }
                 }
             }
-        }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < kLaneNumbers; ++i) v[i] = i < left ? load_as_float(p, type, at + i) : 0.f;
+    for (int u = 0; u < ROWS; ++u)
+#pragma unroll
+        for (int i = 0; i < kLaneNumbers; ++i) v[u][i] = u < n && i < left ? load_as_float(p, TYPE, at[u] + i) : 0.f;
 }
 
 // bits of the largest finite |v|
@@ -139,46 +144,72 @@ struct Fp8Args {
     float* scale;
     int64_t ldx, ldq, T;
     int64_t scale_ld;     // 0: scale [T, C]; else [C, scale_ld] by places in q
-    int32_t K, type, format, E;
-    int32_t warps;        // per row: four blocks each
+    int32_t K, format, E;
+    int32_t parts;        // of a row: four blocks each
     int32_t vec_x, vec_q;
 };
 
-// A warp quantises four blocks of a row: a lane holds 16 consecutive numbers (one 16-byte store), eight lanes a block.
-// Bound by HBM; 32 (64) bytes per lane in flight.  Laid out by bucket: the rows are walked by the plan's tiles.
-template <bool LAID>
-__global__ void __launch_bounds__(kThreads) k_fp8_rows(const __grid_constant__ Fp8Args a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * kWarpsPerCta + (threadIdx.x >> 5);
-    const int64_t r = i / a.warps;
-    const int part = (int)(i - r * a.warps);
-    int64_t from = r, to = r;
+// A warp quantises four blocks of two neighbouring rows: a lane holds 16 consecutive numbers of each (one 16-byte store),
+// eight lanes a block.  A CTA takes 16 rows; the scales go out together, 16 neighbours of a block where they lie by place.
+// Bound by HBM: 16384 x 4096 bf16 in 41 us, 4.9 TB/s (four rows per warp 54 us, too few warps; one 46).  LAID: the rows are
+// walked by the plan's tiles.
+constexpr int kFp8Rows = 2;
+template <int TYPE, bool LAID>
+__global__ void __launch_bounds__(kThreads, 5) k_fp8_rows(const __grid_constant__ Fp8Args a) {
+    constexpr int kCtaRows = kWarpsPerCta * kFp8Rows;
+    __shared__ float s_scale[kWarpNumbers / kFp8Block][kCtaRows + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t group = blockIdx.x / a.parts;
+    const int part = (int)(blockIdx.x - group * a.parts);
+    int64_t to = group * kCtaRows;  // the CTA's first row in q
+    int rows, start = 0;
     if (LAID) {
-        const int64_t t = r / kGroupRows;
+        const int64_t t = group / (kGroupRows / kCtaRows);
         if (t >= __ldg(a.plan.n_tiles)) return;
         const int4 tile = __ldg(reinterpret_cast<const int4*>(a.plan.tiles) + t);
-        const int in = (int)(r - t * kGroupRows);
+        const int in = (int)(group % (kGroupRows / kCtaRows)) * kCtaRows;
         if (tile.x >= a.E || in >= tile.z) return;
-        from = __ldg(a.plan.order + tile.y + in);
+        rows = min(kCtaRows, tile.z - in);
+        start = tile.y + in;
         to = tile.w + in;
-    } else if (r >= a.T) {
-        return;
+    } else {
+        rows = (int)min((int64_t)kCtaRows, a.T - to);
     }
-    const int k = part * kWarpNumbers + lane * kLaneNumbers, C = (a.K + kFp8Block - 1) / kFp8Block;
-    float v[kLaneNumbers];
-    load_sixteen(a.x, a.type, from * a.ldx + k, a.K - k, a.vec_x, v);
-    uint32_t most = largest_bits(v);
+    const int r0 = warp * kFp8Rows, n = min(kFp8Rows, rows - r0);
+    const int k = part * kWarpNumbers + lane * kLaneNumbers, C = (a.K + kFp8Block - 1) / kFp8Block, c = k / kFp8Block;
+    if (n > 0) {
+        int64_t from[kFp8Rows], at[kFp8Rows];
 #pragma unroll
-    for (int d = 1; d < kBlockLanes; d <<= 1) most = max(most, __shfl_xor_sync(kFullMask, most, d));
-    const int e = fp8_scale_exponent(most, a.format);
-    store_sixteen(a.q, to * a.ldq + k, (int)min((int64_t)kLaneNumbers, a.ldq - k), a.vec_q, v, power_of_two(-e), a.format);
-    const int c = k / kFp8Block;
-    if (lane % kBlockLanes == 0 && c < C) a.scale[a.scale_ld ? c * a.scale_ld + to : from * C + c] = power_of_two(e);
+        for (int u = 0; u < kFp8Rows; ++u) {
+            from[u] = u >= n ? 0 : LAID ? (int64_t)__ldg(a.plan.order + start + r0 + u) : to + r0 + u;
+            at[u] = from[u] * a.ldx + k;
+        }
+        float v[kFp8Rows][kLaneNumbers];
+        load_sixteen<TYPE, kFp8Rows>(a.x, at, n, a.K - k, a.vec_x, v);
+#pragma unroll
+        for (int u = 0; u < kFp8Rows; ++u) {
+            uint32_t most = largest_bits(v[u]);
+#pragma unroll
+            for (int d = 1; d < kBlockLanes; d <<= 1) most = max(most, __shfl_xor_sync(kFullMask, most, d));
+            if (u >= n) continue;
+            const int e = fp8_scale_exponent(most, a.format);
+            store_sixteen(a.q, (to + r0 + u) * a.ldq + k, (int)min((int64_t)kLaneNumbers, a.ldq - k), a.vec_q, v[u], power_of_two(-e), a.format);
+            if (lane % kBlockLanes == 0 && c < C) {
+                if (a.scale_ld) s_scale[lane / kBlockLanes][r0 + u] = power_of_two(e);
+                else a.scale[from[u] * C + c] = power_of_two(e);
+            }
+        }
+    }
+    if (!a.scale_ld) return;
+    __syncthreads();
+    const int sc = part * (kWarpNumbers / kFp8Block) + warp;
+    if (warp < kWarpNumbers / kFp8Block && sc < C && lane < rows) a.scale[sc * a.scale_ld + to + lane] = s_scale[warp][lane];
 }
 
 // One CTA per 128 x 128 tile: every number is read once and held in registers, 64 per thread, until the scale is known.
+template <int TYPE>
 __global__ void __launch_bounds__(kThreads, 2)
-    k_fp8_tiles(const void* __restrict__ w, int type, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
+    k_fp8_tiles(const void* __restrict__ w, int64_t ldw, uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale,
                 int64_t N, int64_t K, int format, int vec_w, int vec_q) {
     const int64_t C = (K + kFp8Block - 1) / kFp8Block, R = (N + kFp8Block - 1) / kFp8Block;
     const int64_t tile = blockIdx.x, c = tile % C, r = tile / C % R, e = tile / (C * R);
@@ -186,12 +217,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t n0 = r * kFp8Block + threadIdx.x / kBlockLanes;
     constexpr int kRows = kThreads / kBlockLanes;  // 32 rows at once
     float v[4][kLaneNumbers];
-    uint32_t most = 0;
+    int64_t at[4];
+    const int there = (int)max((int64_t)0, min((int64_t)4, (N - n0 + kRows - 1) / kRows));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + j * kRows;
-        load_sixteen(w, type, (e * N + n) * ldw + k, n < N ? (int)(K - k) : 0, vec_w, v[j]);
-    }
+    for (int j = 0; j < 4; ++j) at[j] = (e * N + n0 + j * kRows) * ldw + k;
+    load_sixteen<TYPE, 4>(w, at, there, (int)(K - k), vec_w, v);
+    uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) most = max(most, largest_bits(v[j]));
     __shared__ uint32_t s_most[kWarpsPerCta];
@@ -202,11 +233,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int j = 0; j < kWarpsPerCta; ++j) most = max(most, s_most[j]);
     const int x = fp8_scale_exponent(most, format);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + j * kRows;
-        if (n < N) store_sixteen(q, (e * N + n) * ldq + k, (int)min((int64_t)kLaneNumbers, ldq - k), vec_q, v[j], power_of_two(-x), format);
-    }
+    for (int j = 0; j < 4; ++j)
+        if (j < there)
+            store_sixteen(q, (e * N + n0 + j * kRows) * ldq + k, (int)min((int64_t)kLaneNumbers, ldq - k), vec_q, v[j], power_of_two(-x), format);
     if (threadIdx.x == 0) scale[tile] = power_of_two(x);
+}
+
+template <int TYPE>
+void launch_fp8_rows(const Fp8Args& a, bool laid, unsigned blocks, cudaStream_t s) {
+    if (laid) k_fp8_rows<TYPE, true><<<blocks, kThreads, 0, s>>>(a);
+    else k_fp8_rows<TYPE, false><<<blocks, kThreads, 0, s>>>(a);
 }
 
 }  // namespace nnue
@@ -244,19 +280,20 @@ extern "C" int nnue_fp8_quantize_rows(const void* x, int32_t type, int64_t ldx, 
     a.scale_ld = scale_ld;
     a.T = T;
     a.K = (int32_t)K;
-    a.type = type;
     a.format = format;
     a.E = E;
-    a.warps = (int32_t)((K + kWarpNumbers - 1) / kWarpNumbers);
+    a.parts = (int32_t)((K + kWarpNumbers - 1) / kWarpNumbers);
     a.vec_x = aligned16(x) && ldx * type_bytes(type) % 16 == 0;
     a.vec_q = aligned16(q) && ldq % 16 == 0;
     const int64_t rows = plan ? group_max_tiles(T, E) * kGroupRows : T;
-    const int64_t blocks = (rows * a.warps + kWarpsPerCta - 1) / kWarpsPerCta;
+    constexpr int kCtaRows = kWarpsPerCta * kFp8Rows;
+    const int64_t blocks = (rows + kCtaRows - 1) / kCtaRows * a.parts;
     NNUE_REQUIRE(blocks <= 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "%s: too many blocks", what);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("fp8_rows", s);
-    if (plan) k_fp8_rows<true><<<(unsigned)blocks, kThreads, 0, s>>>(a);
-    else k_fp8_rows<false><<<(unsigned)blocks, kThreads, 0, s>>>(a);
+    if (type == NNUE_T_F32) launch_fp8_rows<NNUE_T_F32>(a, plan, (unsigned)blocks, s);
+    else if (type == NNUE_T_BF16) launch_fp8_rows<NNUE_T_BF16>(a, plan, (unsigned)blocks, s);
+    else launch_fp8_rows<NNUE_T_F16>(a, plan, (unsigned)blocks, s);
     note_launches(1);
     NNUE_CUDA_TRY(cudaGetLastError());
     return NNUE_OK;
@@ -271,8 +308,9 @@ extern "C" int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw,
     NNUE_REQUIRE(tiles <= 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "nnue_fp8_quantize_tiles: too many tiles");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("fp8_tiles", s);
-    k_fp8_tiles<<<(unsigned)tiles, kThreads, 0, s>>>(w, type, ldw, static_cast<uint8_t*>(q), ldq, scale, N, K, format,
-                                                     aligned16(w) && ldw * type_bytes(type) % 16 == 0, aligned16(q) && ldq % 16 == 0);
+    auto kernel = type == NNUE_T_F32 ? k_fp8_tiles<NNUE_T_F32> : type == NNUE_T_BF16 ? k_fp8_tiles<NNUE_T_BF16> : k_fp8_tiles<NNUE_T_F16>;
+    kernel<<<(unsigned)tiles, kThreads, 0, s>>>(w, ldw, static_cast<uint8_t*>(q), ldq, scale, N, K, format,
+                                                aligned16(w) && ldw * type_bytes(type) % 16 == 0, aligned16(q) && ldq % 16 == 0);
     note_launches(1);
     NNUE_CUDA_TRY(cudaGetLastError());
     return NNUE_OK;
