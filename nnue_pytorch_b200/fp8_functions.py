@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._launch import _outside_graphs, _ptr, _require_cuda, _span, _stream
-from .grouped_linear_functions import GATHERED_ROWS, TYPES, GroupPlan, _on, _pitched
+from .grouped_linear_functions import GATHERED_ROWS, TYPES, GroupPlan, _on, _pitched, _rows
 
 FORMATS = (torch.float8_e4m3fn, torch.float8_e5m2)
 BLOCK = 128
@@ -55,14 +55,6 @@ class Fp8Blocks:
         return self.q.float() * s.reshape(rows, K)
 
 
-def _source(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """(t, pitch) with neighbouring columns next to each other."""
-    t = t.detach()
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _check_source(t: torch.Tensor, format: torch.dtype) -> None:
     assert t.dim() == 2 and t.shape[1] >= 1, "a matrix with at least one column"
     assert t.dtype in (torch.float32, torch.bfloat16, torch.float16), "fp32, bf16 or fp16"
@@ -80,7 +72,7 @@ def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn
     """x [T, K] (fp32, bf16 or fp16) in 8 bits, one scale per 128 consecutive numbers of a row."""
     dev = _require_cuda(x)
     _check_source(x, format)
-    x, ldx = _source(x)
+    x, ldx = _rows(x.detach())
     T, K = x.shape
     q, ldq = _empty_q(T, K, format, dev)
     scale = torch.empty(T, (K + BLOCK - 1) // BLOCK, dtype=torch.float32, device=dev)
@@ -99,7 +91,7 @@ def quantize_fp8_tiles(weight: torch.Tensor, count: int = 1, format: torch.dtype
     _check_source(weight, format)
     count = int(count)
     assert 1 <= count <= 1024 and weight.shape[0] % count == 0, "the matrices' rows do not divide"
-    weight, ldw = _source(weight)
+    weight, ldw = _rows(weight.detach())
     rows, K = weight.shape
     N = rows // count
     assert N >= 1, "empty matrices"
@@ -160,7 +152,7 @@ def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tenso
         wr, ldw = _pitched(weight.q, format, lib, dev)
         C = (K + BLOCK - 1) // BLOCK
         if not given:
-            xs, ldx = _source(x)
+            xs, ldx = _rows(x.detach())
             if laid:
                 nbytes = lib.nnue_group_rows_bytes(T, (K + 15) // 16 * 8, E)
                 xr, pitch, places = torch.empty(nbytes, dtype=torch.uint8, device=dev), 0, nbytes // ((K + 15) // 16 * 16)

@@ -75,6 +75,15 @@ class GroupPlan:
         assert t.device == self.device, "the plan lives on another device"
 
 
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """(t, pitch of its rows) with neighbouring columns next to each other and rows that do not overlap.  The stride of a
+    single row says nothing: a transposed column has 1."""
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        t = t.contiguous()
+    return t, t.stride(0) if rows > 1 else cols
+
+
 def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev, whole: bool = False) -> tuple[torch.Tensor, int]:
     """(t as rows of `dtype` that start at multiples of 16 bytes, their pitch in elements): `t` itself where it is one,
     else a copy whose rows are padded with zeros (`nnue_pack_rows`).  `whole`: the last 16 bytes of every row may be read."""
@@ -88,15 +97,14 @@ def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev, whole: bool = False)
             return t, pitch
         if rows == 1 and cols % unit == 0:
             return t, cols
-    if cols > 1 and t.stride(1) != 1 or t.stride(0) < cols:
-        t = t.contiguous()
+    t, ld = _rows(t)
     pitch = (cols + unit - 1) // unit * unit
     out = torch.empty(rows, pitch, dtype=dtype, device=dev)
     if t.dtype.itemsize != 1:
-        st = lib.nnue_pack_rows(_ptr(t), TYPES[t.dtype], t.stride(0), _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
+        st = lib.nnue_pack_rows(_ptr(t), TYPES[t.dtype], ld, _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
     else:
         assert t.dtype == dtype
-        st = lib.nnue_pack_rows(_ptr(t), TYPES[dtype], t.stride(0), _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
+        st = lib.nnue_pack_rows(_ptr(t), TYPES[dtype], ld, _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
     _lib.check(st, "nnue_pack_rows")
     return out, pitch
 
@@ -104,11 +112,10 @@ def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev, whole: bool = False)
 def _laid_out(t: torch.Tensor, dtype: torch.dtype, plan_buffer, E: int, lib, dev, sums: bool = False):
     """(t laid out by bucket as `dtype` (`nnue_group_rows`), the sums of its columns per tile or None)."""
     T, cols = t.shape
-    if cols > 1 and t.stride(1) != 1 or t.stride(0) < cols:
-        t = t.contiguous()
+    t, ld = _rows(t)
     out = torch.empty(lib.nnue_group_rows_bytes(T, cols, E), dtype=torch.uint8, device=dev)
     part = torch.empty(lib.nnue_group_sums_bytes(T, cols, E) // 4, dtype=torch.float32, device=dev) if sums else None
-    st = lib.nnue_group_rows(_ptr(t), TYPES[t.dtype], t.stride(0), _ptr(plan_buffer), _ptr(out), TYPES[dtype], _ptr(part), T, cols,
+    st = lib.nnue_group_rows(_ptr(t), TYPES[t.dtype], ld, _ptr(plan_buffer), _ptr(out), TYPES[dtype], _ptr(part), T, cols,
                              E, _stream(dev))
     _lib.check(st, "nnue_group_rows")
     return out, part
@@ -208,7 +215,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     bias    count * N numbers of x's type or fp32, or None
     out_dtype  x's type (default) or float32
 
-    Gradients: those of the formula, with dy rounded to x's type where it is fp32; each in its tensor's own type."""
+    Gradients: those of the formula, with dy rounded to x's type where it is fp32; each in its tensor's own type.  They have
+    no gradients of their own.  Everything runs on the current stream and can be captured into a CUDA graph; as for any
+    operator, no eager autograd graph of the same leaves may be alive when a backward pass is captured."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return GroupedLinearFunction.apply(x, weight, bias, plan, out_dtype)
     return _forward(x, weight, bias, plan, out_dtype, False)[0]

@@ -184,6 +184,27 @@ def test_linear_with_unaligned_operands(dev):
     assert torch.equal(linear_fp8(x8, w8, None, plan), linear_fp8(Fp8Blocks(tight(x8.q), x8.scale), w8, None, plan))
 
 
+@pytest.mark.parametrize("format", FORMATS)
+@pytest.mark.parametrize("T,count,K,N", [(3000, 3, 400, 700), (20000, 3, 136, 1000)])
+def test_given_rows_equal_quantised_ones(dev, T, count, K, N, format):
+    """Rows quantised on the way in (scales by block) and rows given with their scales by row: the same bits, also where pairs
+    of SMs share a tile and where rows of no bucket are among them; and the dense product of the same rows."""
+    from nnue_pytorch_b200 import GroupPlan, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
+
+    g = torch.Generator().manual_seed(31)
+    x = (torch.randn(T, K, generator=g) * torch.exp(torch.randn(T, 1, generator=g))).half().to(dev)
+    w8 = quantize_fp8_tiles(torch.randn(count * N, K, generator=g).to(dev), count, format)
+    b = torch.randint(-1, count, (T,), generator=g).to(dev)
+    plan = GroupPlan(b, count)
+    bias = torch.randn(count * N, generator=g).to(dev)
+    y = linear_fp8(x, w8, bias, plan)
+    assert torch.equal(y, linear_fp8(quantize_fp8_rows(x, format), w8, bias, plan, torch.float16))
+    one = quantize_fp8_tiles(torch.randn(N, K, generator=g).to(dev), 1, format)
+    d = linear_fp8(x, one, bias[:N])
+    assert torch.equal(d, linear_fp8(quantize_fp8_rows(x, format), one, bias[:N], None, torch.float16))
+    assert torch.equal(d, linear_fp8(x, one, bias[:N], GroupPlan(torch.zeros(T, dtype=torch.int32, device=dev), 1)))
+
+
 def test_not_finite_rows(dev):
     from nnue_pytorch_b200 import GroupPlan, linear_fp8, quantize_fp8_tiles
 

@@ -28,7 +28,7 @@ def _ids(T, count, seed, padding=False, skew=False):
 # ---- the plan
 @pytest.mark.parametrize("wide", [True, False])
 @pytest.mark.parametrize("T,count", [(0, 3), (1, 1), (1, 1024), (31, 2), (32, 8), (33, 8), (1000, 257), (1025, 1024), (16384, 8),
-                                     (16385, 8), (40961, 5), (70000, 1024)])
+                                     (2048, 3), (2049, 1024), (16385, 8), (40961, 5), (65536, 2), (65537, 700), (70000, 1024)])
 def test_plan(dev, T, count, wide):
     from nnue_pytorch_b200 import GroupPlan
 
@@ -174,6 +174,86 @@ def test_strides_and_alignments(dev):
     x = wide[:, :K].detach().requires_grad_(True)
     grouped_linear(x, wt, None, plan).sum().backward()  # an expanded gradient
     close(x.grad, *linear_ref(x, wt, None, b, count, torch.ones(T, N))["dx"], "dx of a sum")
+
+
+def test_one_row_of_any_stride(dev):
+    """A single row's own stride says nothing: a transposed column has 1."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator().manual_seed(21)
+    plan = GroupPlan(torch.ones(1, dtype=torch.int64, device=dev), 2)
+    for K, N in ((64, 8), (33, 5)):
+        x = torch.randn(K, 1, generator=g).bfloat16().to(dev).t()
+        w = torch.randn(2 * N, K, generator=g).to(dev).requires_grad_(True)
+        dy = torch.randn(N, 1, generator=g).bfloat16().to(dev).t()
+        assert x.stride(0) == 1 and dy.stride(0) == 1
+        b = torch.ones(1, dtype=torch.int64)
+        ref = linear_ref(x, w.detach().bfloat16(), None, b, 2, dy)
+        with torch.no_grad():
+            close(grouped_linear(x, w, None, plan), *ref["y"], "y")
+        xg = x.detach().requires_grad_(True)
+        y = grouped_linear(xg, w, None, plan)
+        dx, dw = torch.autograd.grad(y, (xg, w), dy)
+        close(y, *ref["y"], "y")
+        close(dx, *ref["dx"], "dx")
+        close(dw, *ref["dw"], "dw")
+    w1 = torch.randn(64, 1, generator=g).bfloat16().to(dev).t()  # one output: a weight matrix of one row
+    one = GroupPlan(torch.zeros(3, dtype=torch.int64, device=dev), 1)
+    x = torch.randn(3, 64, generator=g).bfloat16().to(dev)
+    close(grouped_linear(x, w1, None, one), *linear_ref(x, w1, None, torch.zeros(3, dtype=torch.int64), 1)["y"], "one output")
+
+
+def test_inside_a_compiled_model(dev):
+    """The calls run eagerly inside a function that torch.compile traces, with their gradients."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator().manual_seed(22)
+    b = _ids(200, 4, 22, padding=True).to(dev)
+    plan = GroupPlan(b, 4)
+    x = torch.randn(200, 48, generator=g).bfloat16().to(dev).requires_grad_(True)
+    w = torch.randn(4 * 24, 48, generator=g).to(dev).requires_grad_(True)
+
+    def layer(x, w):
+        return grouped_linear(x * 2, w, None, plan).clamp(0, 1) * 3
+
+    want = layer(x, w)
+    got = torch.compile(layer, backend="eager")(x, w)
+    assert torch.equal(want, got)
+    for p, q in zip(torch.autograd.grad(want.sum(), (x, w)), torch.autograd.grad(got.sum(), (x, w))):
+        assert torch.equal(p, q)
+
+
+def test_trained_layers_then_evaluated_in_8_bits(dev):
+    """One plan through two bucketed layers, forward and backward, then the same layers exported to 8 bits.
+
+    With dyadic inputs (multiples of 1/4 of at most 1, weights of -1, 0, 1 over 8, few terms) every sum and every rounding
+    on the way is exact, in 16 and in 8 bits: both paths have to equal the 64-bit network to the bit."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear, linear_fp8, quantize_fp8_tiles
+
+    g = torch.Generator().manual_seed(23)
+    T, count, K, H, N = 5000, 8, 160, 40, 16
+    b = _ids(T, count, 23, padding=True)
+    x = torch.randint(0, 5, (T, K), generator=g) / 4 * (torch.rand(T, K, generator=g) < 0.05)
+    w1 = torch.randint(-1, 2, (count * H, K), generator=g) / 4.0
+    w2 = torch.randint(-1, 2, (count * N, H), generator=g) / 4.0
+    plan = GroupPlan(b.to(dev), count)
+    clip = lambda t: (t * 4).round().clamp(0, 4) / 4  # noqa: E731  an activation on the same quarters
+
+    h64 = clip(linear_ref(x, w1, None, b, count)["y"][0])
+    ref = linear_ref(h64, w2, None, b, count, torch.ones(T, N))
+    xd = x.bfloat16().to(dev)
+    w1d, w2d = w1.to(dev), w2.to(dev).requires_grad_(True)
+    h = clip(grouped_linear(xd, w1d, None, plan))
+    assert torch.equal(h.cpu().double(), h64)
+    y = grouped_linear(h, w2d, None, plan, out_dtype=torch.float32)
+    assert torch.equal(y.detach().cpu().double(), ref["y"][0])
+    dw, = torch.autograd.grad(y.sum(), w2d)
+    assert torch.equal(dw.cpu().double(), ref["dw"][0])
+    with torch.no_grad():
+        a = clip(linear_fp8(xd, quantize_fp8_tiles(w1d, count), None, plan))
+        assert torch.equal(a, h)
+        e = linear_fp8(a, quantize_fp8_tiles(w2d, count), None, plan, out_dtype=torch.float32)
+    assert torch.equal(e, y.detach())
 
 
 def test_not_finite_values_stay_where_they_are(dev):
