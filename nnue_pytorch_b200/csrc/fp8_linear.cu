@@ -242,7 +242,7 @@ __device__ __forceinline__ void f8_bring_out(const F8Args& a, const F8Tile& x, f
             for (int p = 0; p < 8; ++p)
                 *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
                     make_float4(acc[h + 4 * p], acc[h + 4 * p + 1], acc[h + 4 * p + 2], acc[h + 4 * p + 3]);
-            copy_rows_out(a.o, stg, 128, my_row, 0, col + h);
+            copy_rows_out<128>(a.o, stg, my_row, 0, col + h);
         }
     } else {
         constexpr int kPass = HALF < 64 ? HALF : 64;
@@ -255,7 +255,7 @@ __device__ __forceinline__ void f8_bring_out(const F8Args& a, const F8Tile& x, f
                 for (int j = 0; j < 4; ++j) w[j] = pack_half(acc[h + 8 * p + 2 * j], acc[h + 8 * p + 2 * j + 1], a.o.type);
                 *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            copy_rows_out(a.o, stg, kPass * 2, my_row, 0, col + h);
+            copy_rows_out<kPass * 2>(a.o, stg, my_row, 0, col + h);
         }
     }
 }

@@ -114,43 +114,47 @@ __device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bo
     const bool wide = !f32 && BN >= 64;  // two reads of 32 columns make one 128-byte piece of a row
 #pragma unroll 1
     for (int c = 0; c < BN && col0 + c < a.o.cols; c += wide ? 64 : 32) {
-#pragma unroll 1
-        for (int h = 0; h < (wide ? 2 : 1); ++h) {
-            uint32_t v[32];
-            if (zeros) {
+        uint32_t v[2][32];
+        if (zeros) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0u;
-            } else {
-                tmem_ld32(taddr + c + 32 * h, v);
-                tmem_wait_ld();
-                if (s_bias) {
+            for (int j = 0; j < 64; ++j) v[j / 32][j % 32] = 0u;
+        } else {  // both reads under way before the wait
+            tmem_ld32(taddr + c, v[0]);
+            if (wide) tmem_ld32(taddr + c + 32, v[1]);
+            tmem_wait_ld(v[0]);
+            if (wide) tmem_wait_ld(v[1]);
+        }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 b = *reinterpret_cast<const float4*>(s_bias + c + 32 * h + j);
-                        v[j] = __float_as_uint(__uint_as_float(v[j]) + b.x);
-                        v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b.y);
-                        v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b.z);
-                        v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + b.w);
-                    }
+        for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !wide) break;
+            if (s_bias && !zeros) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(s_bias + c + 32 * h + j);
+                    v[h][j] = __float_as_uint(__uint_as_float(v[h][j]) + b.x);
+                    v[h][j + 1] = __float_as_uint(__uint_as_float(v[h][j + 1]) + b.y);
+                    v[h][j + 2] = __float_as_uint(__uint_as_float(v[h][j + 2]) + b.z);
+                    v[h][j + 3] = __float_as_uint(__uint_as_float(v[h][j + 3]) + b.w);
                 }
             }
             if (f32) {
 #pragma unroll
                 for (int p = 0; p < 8; ++p)
                     *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
-                        make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+                        make_uint4(v[h][4 * p], v[h][4 * p + 1], v[h][4 * p + 2], v[h][4 * p + 3]);
             } else {
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
                     uint32_t w[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        w[j] = pack_half(__uint_as_float(v[8 * p + 2 * j]), __uint_as_float(v[8 * p + 2 * j + 1]), a.o.type);
+                        w[j] = pack_half(__uint_as_float(v[h][8 * p + 2 * j]), __uint_as_float(v[h][8 * p + 2 * j + 1]), a.o.type);
                     *reinterpret_cast<uint4*>(stg + lane * 128 + (((4 * h + p) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
-        copy_rows_out(a.o, stg, f32 || wide ? 128 : 64, my_row, row_base, col0 + c);
+        if (f32 || wide) copy_rows_out<128>(a.o, stg, my_row, row_base, col0 + c);
+        else copy_rows_out<64>(a.o, stg, my_row, row_base, col0 + c);
     }
 }
 

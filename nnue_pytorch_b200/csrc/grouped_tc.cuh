@@ -53,31 +53,37 @@ struct StageRing {
     }
 };
 
-// A pass of columns (`bytes` per row in the warp's staging, 16-byte pieces swizzled) to the rows of the output, in whole
-// 128- or 64-byte pieces of rows.  Lane r holds row r's place in the output, or -1.
-__device__ __forceinline__ void copy_rows_out(const RowsOut& o, const unsigned char* stg, int bytes, int32_t my_row, int64_t row_base,
-                                            int col) {
+// A pass of columns (BYTES per row in the warp's staging, 16-byte pieces swizzled) to the rows of the output, in whole
+// 128- or 64-byte pieces of rows.  Lane r holds row r's place in the output, or -1.  The places and the pieces are fetched
+// before the first store: one after the other they cost a warp 800 cycles per pass, more than reading the accumulator.
+template <int BYTES>
+__device__ __forceinline__ void copy_rows_out(const RowsOut& o, const unsigned char* stg, int32_t my_row, int64_t row_base, int col) {
     const int lane = threadIdx.x & 31;
     const int es = o.type == NNUE_T_F32 ? 4 : 2;
     unsigned char* out = static_cast<unsigned char*>(o.out);
     __syncwarp();
     if (o.vec) {
-        const int shift = bytes == 128 ? 3 : 2, piece = lane & ((1 << shift) - 1);
+        constexpr int kShift = BYTES == 128 ? 3 : 2, kRows = 32 >> kShift, kPasses = 32 / kRows;  // kRows: rows at once
+        const int piece = lane & ((1 << kShift) - 1);
         const bool inside = col + piece * (16 / es) < o.cols;  // cols is a multiple of a piece
+        int32_t row[kPasses];
+        uint4 v[kPasses];
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-            const int r = (it << (5 - shift)) + (lane >> shift);
-            const int32_t row = __shfl_sync(kFullMask, my_row, r & 31);
-            if (r >= 32 || row < 0 || !inside) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
-            *reinterpret_cast<uint4*>(out + ((row_base + row) * o.ld + col) * es + piece * 16) = v;
+        for (int it = 0; it < kPasses; ++it) row[it] = __shfl_sync(kFullMask, my_row, it * kRows + (lane >> kShift));
+#pragma unroll
+        for (int it = 0; it < kPasses; ++it) {
+            const int r = it * kRows + (lane >> kShift);
+            v[it] = *reinterpret_cast<const uint4*>(stg + r * 128 + ((piece ^ (r & 7)) << 4));
         }
+#pragma unroll
+        for (int it = 0; it < kPasses; ++it)
+            if (row[it] >= 0 && inside) *reinterpret_cast<uint4*>(out + ((row_base + row[it]) * o.ld + col) * es + piece * 16) = v[it];
     } else {
 #pragma unroll 1
         for (int r = 0; r < 32; ++r) {
             const int32_t row = __shfl_sync(kFullMask, my_row, r);
             if (row < 0) continue;
-            for (int j = lane; j < bytes / es && col + j < o.cols; j += 32) {
+            for (int j = lane; j < BYTES / es && col + j < o.cols; j += 32) {
                 const unsigned char* src = stg + r * 128 + (((j * es / 16) ^ (r & 7)) << 4) + j * es % 16;
                 unsigned char* dst = out + ((row_base + row) * o.ld + col + j) * es;
                 if (es == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
