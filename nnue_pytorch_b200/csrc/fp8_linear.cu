@@ -3,11 +3,14 @@
 //   y[p, n] = sum_c sx[p, c] sw[b, n / 128, c] sum_{k in block c} x[p, k] w[b, n, k] + bias[b, n]
 //
 // A stage is one block of 128 inputs (a 128-byte swizzle row per operand row), four tcgen05.mma of 32 inputs each, whose
-// sum goes to an accumulator of its own in tensor memory; eight warps take the accumulators one after the other, multiply
-// them by sx * sw and add them up in fp32 registers (a thread holds half a row of the tile: its row's scale is one number,
-// and so is the weights' on its columns).  The scales may be any fp32 numbers.  The tensor core takes 512 cycles for a
-// stage of 128 x 256, reading the accumulator 256, the multiply-adds 256 issue slots of each quarter: they overlap, two
-// accumulators (four of 128 columns) being in turn.
+// sum goes to an accumulator of its own in tensor memory.  Eight warps take the accumulators one after the other, multiply
+// them by sx * sw and add them up in fp32 registers (a thread holds half a row of the tile; its row's scale is one number,
+// and so is the weights' on its columns); another warp fetches the scales, which may be any fp32 numbers.
+// Bound by the way of an accumulator, not by the tensor core: a stage of a pair of SMs on 256 x 256 multiplies in 390 cycles,
+// but its first result is there after 900, is read and scaled in 700 to 900 and given back in 240, and tensor memory holds
+// two: about 1000 cycles per stage (16384 x 4096 x 2048 over 8 buckets: 179 us, 1.54 PFLOP/s; 100 us of it are stages at
+// work, 40 the bringing out of eight tiles per pair).  Four accumulators of 128 columns halve the way but double the stages
+// (223 us), and two products of 128 columns per stage came to 219.
 // Copies, pairs of SMs, split sums and bounded waits as in the 16-bit kernel (grouped_linear.cu).  Rows come laid out by
 // bucket (the quantiser leaves them so), in their own order where there is one matrix, or are gathered by TMA, four per
 // copy, where a bucket has few.

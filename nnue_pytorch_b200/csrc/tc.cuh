@@ -236,8 +236,9 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
     return r;
 }
-// On another CTA's barrier, for reads of tensor memory that tc_fence_before has closed.  (A release of cluster scope waits
-// for all of the warp's memory traffic: 8-bit product of 16384 x 4096 x 2048, one arrival per stage and warp, 330 us; so 178.)
+// On another CTA's barrier, after reads of tensor memory that tc_fence_before has closed: nothing else has to be visible
+// there, so it is relaxed.  (A release of cluster scope waits for all of the warp's memory traffic: 330 us for the 8-bit
+// product of 16384 x 4096 x 2048, one arrival per stage and warp, against 178.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
