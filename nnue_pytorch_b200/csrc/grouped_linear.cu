@@ -14,7 +14,7 @@
 // 4096 x 2048), and rows gathered by 16-byte asynchronous copies came to 36 GB/s per SM with four warps (254 us; 595 for
 // dw): laying the rows out first costs 42 us there, and both directions read them.
 //
-// Roles: warp 0 copies into a ring of stages, one thread of warp 1 issues the instructions, warps 2-5 bring finished
+// Roles: warp 0 copies into a ring of stages, warp 1 issues the instructions, warps 2-9 bring finished
 // tiles out while the next tile multiplies (two accumulators).  Persistent: a CTA (or pair) per SM walks the tiles with
 // a stride of the grid.
 // CTAS = 2: a pair of SMs works on 256 rows x BN columns, each holding its half of A and of B: half the bytes of B per
@@ -38,14 +38,15 @@ enum { kModeFwd = 0, kModeDx = 1, kModeDw = 2 };
 constexpr int kGlK = 64;                     // reduction elements per stage: one 128-byte swizzle row
 constexpr int kGlABytes = kGroupRows * 128;  // 16 KiB
 constexpr int kGlBoxBytes = kGlK * 128;      // MN-major block: 64 rows of the reduction x 128 bytes
-constexpr int kGlThreads = 192;
+constexpr int kGlThreads = 320;
 constexpr int kGlLong = 8;                   // stages between additions to the total
 
 constexpr int gl_stage_bytes(int bn, int ctas) { return kGlABytes + bn / ctas * 128; }
 constexpr int gl_stages(int bn, int ctas) { return gl_stage_bytes(bn, ctas) > 32768 ? 4 : gl_stage_bytes(bn, ctas) > 24576 ? 6 : 8; }
-constexpr int gl_smem(int bn, int ctas) {  // alignment, ring, staging, bias per output warp, barriers
-    return 1024 + gl_stages(bn, ctas) * gl_stage_bytes(bn, ctas) + 4 * kStagingBytes + 4 * bn * 4 + 256;
+constexpr int gl_smem(int bn, int ctas) {  // alignment, ring, staging, barriers
+    return 1024 + gl_stages(bn, ctas) * gl_stage_bytes(bn, ctas) + 8 * kStagingBytes + 256;
 }
+constexpr int gl_warp_cols(int bn) { return bn >= 64 ? bn / 2 : bn; }  // columns of an output warp
 
 struct GlArgs {
     GroupPlanView plan;
@@ -107,15 +108,33 @@ __device__ __forceinline__ int gl_steps(const GlArgs& a, const GlTile& x, int c)
     return left >= kGlK ? 4 : (left + 15) >> 4;
 }
 
-// One output warp: its 32 rows of the tile, from tensor memory (or zeros) to the output.
-template <int BN>
-__device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bool zeros, const float* s_bias, unsigned char* stg,
+// One output warp: its 32 rows and COLS columns of the tile, from tensor memory (or zeros) to the output.  `bias`: where the
+// warp's first column's is, or null.
+template <int COLS>
+__device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bool zeros, bool biased, int64_t bias_at, unsigned char* stg,
                                              int32_t my_row, int64_t row_base, int col0) {
     const int lane = threadIdx.x & 31;
     const bool f32 = a.o.type == NNUE_T_F32;
-    const bool wide = !f32 && BN >= 64;  // two reads of 32 columns make one 128-byte piece of a row
+    const bool wide = !f32 && COLS >= 64;  // two reads of 32 columns make one 128-byte piece of a row
+    const int step = wide ? 64 : 32;
+    float* s_bias = reinterpret_cast<float*>(stg);
+    float next[2] = {0.f, 0.f};  // bias of the next columns, on its way while these go out
+    auto fetch = [&](int c) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int j = c + 32 * h + lane;
+            next[h] = 32 * h < step && j < COLS && col0 + j < a.o.cols ? load_as_float(a.bias, a.bias_type, bias_at + j) : 0.f;
+        }
+    };
+    if (biased) fetch(0);
 #pragma unroll 1
-    for (int c = 0; c < BN && col0 + c < a.o.cols; c += wide ? 64 : 32) {
+    for (int c = 0; c < COLS && col0 + c < a.o.cols; c += step) {
+        if (biased) {
+            s_bias[lane] = next[0];
+            s_bias[32 + lane] = next[1];
+            fetch(c + step);
+            __syncwarp();
+        }
         uint32_t v[2][32];
         if (zeros) {
 #pragma unroll
@@ -126,19 +145,24 @@ __device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bo
             tmem_wait_ld(v[0]);
             if (wide) tmem_wait_ld(v[1]);
         }
+        if (biased) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (h == 1 && !wide) break;
-            if (s_bias && !zeros) {
+            for (int h = 0; h < 2; ++h) {
+                if (h == 1 && !wide) break;
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
-                    const float4 b = *reinterpret_cast<const float4*>(s_bias + c + 32 * h + j);
+                    const float4 b = *reinterpret_cast<const float4*>(s_bias + 32 * h + j);
                     v[h][j] = __float_as_uint(__uint_as_float(v[h][j]) + b.x);
                     v[h][j + 1] = __float_as_uint(__uint_as_float(v[h][j + 1]) + b.y);
                     v[h][j + 2] = __float_as_uint(__uint_as_float(v[h][j + 2]) + b.z);
                     v[h][j + 3] = __float_as_uint(__uint_as_float(v[h][j + 3]) + b.w);
                 }
             }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !wide) break;
             if (f32) {
 #pragma unroll
                 for (int p = 0; p < 8; ++p)
@@ -271,10 +295,10 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
 }
 
 // One output warp: total (+)= accumulator, its 32 lanes.
-template <int BN>
+template <int COLS>
 __device__ __forceinline__ void gl_add_to_total(uint32_t acc, uint32_t total, bool first) {
 #pragma unroll 1
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = 0; c < COLS; c += 32) {
         uint32_t v[32], w[32];
         tmem_ld32(acc + c, v);
         if (!first) {
@@ -311,8 +335,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
     unsigned char* staging = ring_ptr + S * gl_stage_bytes(BN, CTAS);
-    float* s_bias = reinterpret_cast<float*>(staging + 4 * kStagingBytes);  // [4][BN], one copy per output warp
-    uint64_t* full = reinterpret_cast<uint64_t*>(s_bias + 4 * BN);         // [S] a stage's copies are in (pair: the first CTA's)
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * kStagingBytes);  // [S] a stage's copies are in (pair: the first CTA's)
     uint64_t* empty = full + S;                                            // [S] a stage may be overwritten
     uint64_t* done = empty + S;                                            // [2] an accumulator is complete
     uint64_t* taken = done + 2;                                            // [2] an accumulator has been read
@@ -338,7 +361,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(done + s, 1);
-            mbar_init(taken + s, 4 * CTAS);
+            mbar_init(taken + s, 8 * CTAS);
         }
         mbar_init(drained, 1);
         fence_barrier_init();
@@ -359,9 +382,10 @@ __global__ void __launch_bounds__(kGlThreads, 1)
         if (!(PAIR && rank != 0))
             ok = gl_issue_role<MODE, BN, CTAS, SPLIT, LONG>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
     } else {
-        const int q = warp & 3;  // the quarter of tensor memory's lanes that this warp may read
-        const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        float* my_bias = s_bias + q * BN;
+        constexpr int kCols = gl_warp_cols(BN);
+        const int q = warp & 3, half = (warp - 2) >> 2;  // the quarter of tensor memory's lanes, the half of the columns
+        const bool works = half * kCols < BN;            // 32 columns are one half
+        const uint32_t lanes = ((uint32_t)(q * 32) << 16) + half * kCols;
         StageRing<2> acc;
         for (int t = t0; t < tiles && ok; t += stride) {
             const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
@@ -372,16 +396,11 @@ __global__ void __launch_bounds__(kGlThreads, 1)
             if (MODE == kModeDw) {
                 my_row = x.row0 + r < a.N ? x.row0 + r : -1;
                 row_base = (int64_t)x.bucket * a.N;
-                if (!SPLIT && a.sums && x.col0 == 0 && my_row >= 0) gl_bias_gradient(a, x, my_row);
+                if (!SPLIT && a.sums && x.col0 == 0 && half == 0 && my_row >= 0) gl_bias_gradient(a, x, my_row);
             } else {
                 my_row = r < x.count ? __ldg(a.plan.order + x.first + r) : -1;
             }
             const bool biased = MODE == kModeFwd && !SPLIT && a.bias && x.live;
-            if (biased) {
-                for (int j = lane; j < BN; j += 32)
-                    my_bias[j] = x.col0 + j < a.o.cols ? load_as_float(a.bias, a.bias_type, (int64_t)x.bucket * a.N + x.col0 + j) : 0.f;
-                __syncwarp();
-            }
             auto give_back = [&] {
                 tc_fence_before();
                 __syncwarp();
@@ -397,7 +416,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
                     ok = mbar_wait_warp(done + acc.stage, acc.phase);
                     if (!ok) break;
                     tc_fence_after();
-                    gl_add_to_total<BN>(tmem + lanes + acc.stage * BN, tmem + lanes + 2 * BN, g == x.c0);
+                    if (works) gl_add_to_total<kCols>(tmem + lanes + acc.stage * BN, tmem + lanes + 2 * BN, g == x.c0);
                     give_back();
                 }
                 from = tmem + lanes + 2 * BN;
@@ -406,8 +425,10 @@ __global__ void __launch_bounds__(kGlThreads, 1)
                 if (ok) tc_fence_after();
             }
             if (!ok || SPLIT) break;
-            if (__any_sync(kFullMask, my_row >= 0))
-                gl_bring_out<BN>(a, from, !some, biased ? my_bias : nullptr, staging + q * kStagingBytes, my_row, row_base, x.col0);
+            const int col = x.col0 + half * kCols;
+            if (works && __any_sync(kFullMask, my_row >= 0))
+                gl_bring_out<kCols>(a, from, !some, biased && some, (int64_t)x.bucket * a.N + col, staging + (warp - 2) * kStagingBytes, my_row,
+                                    row_base, col);
             if (!LONG && some) give_back();
         }
     }
@@ -418,10 +439,10 @@ __global__ void __launch_bounds__(kGlThreads, 1)
         __syncthreads();  // nobody reads the ring any more: the partial tile takes its place
         const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t0, rank, ranks);
         if (warp >= 2) {
-            const int q = warp & 3;
+            const int q = warp & 3, half = (warp - 2) >> 2;
             float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * kPartPitch;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
+            for (int c = half * gl_warp_cols(BN); c < min(BN, (half + 1) * gl_warp_cols(BN)); c += 32) {
                 uint32_t v[32];
                 if (x.c1 > x.c0) {
                     tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (LONG ? 2 * BN : 0) + c, v);
