@@ -8,8 +8,8 @@
 // and so is the weights' on its columns); another warp fetches the scales, which may be any fp32 numbers.
 // Bound by the way of an accumulator, not by the tensor core: a stage of a pair of SMs on 256 x 256 multiplies in 390 cycles,
 // but its first result is there after 900, is read and scaled in 700 to 900 and given back in 240, and tensor memory holds
-// two: about 1000 cycles per stage (16384 x 4096 x 2048 over 8 buckets: 179 us, 1.54 PFLOP/s; 100 us of it are stages at
-// work, 40 the bringing out of eight tiles per pair).  Four accumulators of 128 columns halve the way but double the stages
+// two: about 1000 cycles per stage (16384 x 4096 x 2048 over 8 buckets: 175 us, 1.57 PFLOP/s; 135 us of it are stages at
+// work, 20 to 40 the bringing out of eight tiles per pair).  Four accumulators of 128 columns halve the way but double the stages
 // (223 us), and two products of 128 columns per stage came to 219.
 // Copies, pairs of SMs, split sums and bounded waits as in the 16-bit kernel (grouped_linear.cu).  Rows come laid out by
 // bucket (the quantiser leaves them so), in their own order where there is one matrix, or are gathered by TMA, four per
@@ -505,7 +505,7 @@ int f8_launch(const CUtensorMap& mx, const CUtensorMap& mw, const F8Args& a, int
 
 // Pairs on 256 columns or CTAs on up to 128.  A round of the latter takes about 5/8 of a pair's round for half the work: at
 // 4099 x 2000 x 1500 two rounds of pairs, 1.4 full, came to 55 us and three of single CTAs, 2.7 full, to 50; at 16384 x 4096
-// x 2048 over 8 buckets eight rounds of pairs to 178 us, against 223 for pairs on 128 columns.
+// x 2048 over 8 buckets eight rounds of pairs to 175 us, against 223 for pairs on 128 columns.
 static TileShape f8_shape(int64_t runs, int64_t T, int64_t N, int64_t chunks, bool pairs) {
     const int64_t rows = (T + runs - 1) / runs, sms = sm_count();
     auto rounds = [&](int64_t high, int64_t wide, int64_t at_once) {

@@ -25,7 +25,7 @@
 // LONG (dw in fp32): the tensor core's adder cuts off, so an error grows with the number of additions (2.4e-6 of the
 //   gradient at 2048 rows).  Every 512 rows the accumulator is added, rounding to nearest, to a total that also lives in
 //   tensor memory.
-// Measured at 16384 x 4096 x 2048 over 8 buckets, bf16: forward 180 us (1.53 PFLOP/s), dx 207, dw 226 after 41 us for laying
+// Measured at 16384 x 4096 x 2048 over 8 buckets, bf16: forward 180 us (1.53 PFLOP/s), dx 198, dw 226 after 41 us for laying
 //   x out and 20 for dy; the operands' way through L2 and shared memory bounds all three (32 KB per SM and stage).
 // All orders are fixed by the sizes: results are reproducible.  Every wait is bounded; one that runs out raises the
 // device status word and the CTA leaves, its tensor memory freed; copies in flight are then as old as that wait.
