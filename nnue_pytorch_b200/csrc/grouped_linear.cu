@@ -303,11 +303,12 @@ __device__ __forceinline__ void gl_add_to_total(uint32_t acc, uint32_t total, bo
         tmem_ld32(acc + c, v);
         if (!first) {
             tmem_ld32(total + c, w);
-            tmem_wait_ld();
+            tmem_wait_ld(v);
+            tmem_wait_ld(w);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
         } else {
-            tmem_wait_ld();
+            tmem_wait_ld(v);
         }
         tmem_st32(total + c, v);
     }
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(kGlThreads, 1)
                 uint32_t v[32];
                 if (x.c1 > x.c0) {
                     tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (LONG ? 2 * BN : 0) + c, v);
-                    tmem_wait_ld();
+                    tmem_wait_ld(v);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0u;

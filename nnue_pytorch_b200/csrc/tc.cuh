@@ -200,7 +200,8 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// the same, naming the registers: nothing that uses them moves before the wait
+// Names the registers that the reads fill, one call per read: a wait that names none orders memory, and arithmetic on the
+// registers may still be placed before it.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
@@ -219,7 +220,6 @@ template <int N>
 __device__ __forceinline__ void more_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---- clusters -----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
