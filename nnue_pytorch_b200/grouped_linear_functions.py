@@ -126,8 +126,8 @@ GATHERED_ROWS = 16
 
 
 def _forward(x, weight, bias, plan, out_dtype, keep_rows):
-    """y, x as the product read it, the weights as it read them and their pitch.  `keep_rows`: x is laid out by bucket whatever
-    its length, as the weight gradient reads it."""
+    """y, x as the product read it and the weights as it read them.  `keep_rows`: x is laid out by bucket whatever its
+    length, as the weight gradient reads it."""
     dev = _require_cuda(x, weight) if bias is None else _require_cuda(x, weight, bias)
     dtype = x.dtype
     assert dtype in HALF, "rows are bf16 or fp16"
@@ -159,15 +159,15 @@ def _forward(x, weight, bias, plan, out_dtype, keep_rows):
             _ptr(xr), ldx, laid, _ptr(wr), ldw, _ptr(bias), 0 if bias is None else TYPES[bias.dtype], _ptr(plan.buffer), _ptr(y),
             TYPES[out_dtype], T, K, N, E, TYPES[dtype], s)
     _lib.check(st, "nnue_grouped_linear_fwd")
-    return y, xr, wr, ldw
+    return y, xr, wr
 
 
 class GroupedLinearFunction(autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, plan, out_dtype=None):
-        y, xr, wr, ldw = _forward(x, weight, bias, plan, out_dtype, ctx.needs_input_grad[1])
+        y, xr, wr = _forward(x, weight, bias, plan, out_dtype, ctx.needs_input_grad[1])
         ctx.save_for_backward(xr if ctx.needs_input_grad[1] else None, wr if ctx.needs_input_grad[0] else None, plan.buffer)
-        ctx.dims = (*x.shape, y.shape[1], plan.count, ldw)
+        ctx.dims = (*x.shape, y.shape[1], plan.count)
         ctx.dtype, ctx.w_like, ctx.b_like = x.dtype, (weight.dtype, weight.shape), None if bias is None else (bias.dtype, bias.shape)
         return y
 
@@ -175,13 +175,15 @@ class GroupedLinearFunction(autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, plan = ctx.saved_tensors
-        T, K, N, E, ldw = ctx.dims
+        T, K, N, E = ctx.dims
         dev, dtype = dy.device, ctx.dtype
         lib = _lib.load()
         need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         dx = dw = db = None
         with _on(dev), _span("grouped_linear_bwd", dev):
             s = _stream(dev)
+            # saved-tensor hooks may give the same numbers back with other strides
+            plan, x = plan.contiguous(), None if x is None else x.contiguous()
             if need_w or need_b or T > GATHERED_ROWS * E:
                 dyr, part = _laid_out(dy, dtype, plan, E, lib, dev, sums=need_b)
                 laid, lddy = 1, 0
@@ -189,6 +191,7 @@ class GroupedLinearFunction(autograd.Function):
                 dyr, lddy = _pitched(dy, dtype, lib, dev)
                 laid = 0
             if need_x:
+                w, ldw = _pitched(w, dtype, lib, dev)
                 dx = torch.empty(T, K, dtype=dtype, device=dev)
                 _lib.check(lib.nnue_grouped_linear_bwd_input(_ptr(dyr), lddy, laid, _ptr(w), ldw, _ptr(plan), _ptr(dx), T, K, N, E,
                                                              TYPES[dtype], s), "nnue_grouped_linear_bwd_input")

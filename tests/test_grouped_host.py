@@ -1,7 +1,75 @@
 """Host side of the bucketed and 8-bit operators, without a GPU: what the C entries are called with, and rules on the sources."""
 
+import contextlib
 import re
+import types
 from pathlib import Path
+
+import pytest
+import torch
+
+
+class _Recorder:
+    """In place of the native library: sizes that are large enough, and the arguments of every launch."""
+
+    def __init__(self):
+        self.calls = {}
+
+    def __getattr__(self, name):
+        if name.endswith("_bytes"):
+            return lambda *args: 1 << 16
+        return lambda *args: self.calls.setdefault(name, []).append(args) or 0
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    """`grouped_linear` on CPU tensors: its checks and its calls, no kernel."""
+    from nnue_pytorch_b200 import grouped_linear_functions as gl
+
+    lib = _Recorder()
+    monkeypatch.setattr(gl._lib, "load", lambda: lib)
+    monkeypatch.setattr(gl, "_require_cuda", lambda *tensors: tensors[0].device)
+    monkeypatch.setattr(gl, "_on", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(gl, "_stream", lambda dev: 0)
+    return lib
+
+
+def _plan(rows, count):
+    return types.SimpleNamespace(rows=rows, count=count, buffer=torch.zeros(1 << 14, dtype=torch.int32), check=lambda t: None)
+
+
+@pytest.mark.parametrize("rows", [4, 400])  # gathered, and laid out by bucket
+@pytest.mark.parametrize("hooks", ["none", "contiguous", "columns"])
+def test_backward_reads_the_weights_at_the_pitch_they_have(recorder, rows, hooks):
+    """Saved-tensor hooks may give a column slice of the weights back with other strides than it was saved with."""
+    from nnue_pytorch_b200 import grouped_linear
+
+    count, N, K = 2, 8, 64
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, requires_grad=True)
+    wide = torch.zeros(count * N, 2 * K, dtype=torch.bfloat16)
+    seen = []
+
+    def columns(t):  # column-major, where it is a matrix
+        seen.append(t.t().contiguous().t() if t.dim() == 2 else t)
+        return seen[-1]
+
+    def tight(t):
+        seen.append(t.contiguous().clone())
+        return seen[-1]
+
+    unpack = {"contiguous": tight, "columns": columns}.get(hooks)
+    context = contextlib.nullcontext() if unpack is None else torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack)
+    with context:
+        y = grouped_linear(x, wide[:, :K], None, _plan(rows, count))
+    assert recorder.calls["nnue_grouped_linear_fwd"][0][4] == 2 * K  # the slice itself was read
+    y.backward(torch.zeros(rows, N, dtype=torch.bfloat16))
+    address, pitch = recorder.calls["nnue_grouped_linear_bwd_input"][0][3:5]
+    if hooks == "none":
+        assert (address, pitch) == (wide.data_ptr(), 2 * K)
+    elif hooks == "contiguous":
+        assert address in [t.data_ptr() for t in seen] and pitch == K
+    else:  # rows of one number next to each other: a copy of tight rows
+        assert address not in [t.data_ptr() for t in seen] and pitch == K
 
 
 def test_waits_for_tensor_memory_name_their_registers():
