@@ -579,7 +579,7 @@ extern "C" int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid, con
     const int64_t tiles = (plan ? group_max_tiles(T, E) : (T + kGroupRows - 1) / kGroupRows) * a.col_tiles;
     NNUE_REQUIRE(tiles * 8 < 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "%s: too many tiles", what);
     if (shape.ctas == 2) return f8_launch<256, 2, false>(mx, mw, a, tiles, 1, s);
-    const bool split = shape.ranks > 1;
-    if (shape.bn == 64) return split ? f8_launch<64, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<64, 1, false>(mx, mw, a, tiles, 1, s);
-    return split ? f8_launch<128, 1, true>(mx, mw, a, tiles, shape.ranks, s) : f8_launch<128, 1, false>(mx, mw, a, tiles, 1, s);
+    if (shape.ranks > 1) return f8_launch<64, 1, true>(mx, mw, a, tiles, shape.ranks, s);
+    if (shape.bn == 64) return f8_launch<64, 1, false>(mx, mw, a, tiles, 1, s);
+    return f8_launch<128, 1, false>(mx, mw, a, tiles, 1, s);
 }

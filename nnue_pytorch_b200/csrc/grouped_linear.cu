@@ -542,18 +542,11 @@ int gl_run(const CUtensorMap& ma, const CUtensorMap& mb, GlArgs& a, int64_t tile
     const int64_t tiles = tile_rows * a.col_tiles;
     NNUE_REQUIRE(tiles * 8 < 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "grouped linear: too many tiles");
     if (shape.ctas == 2) return gl_launch<MODE, kWidest, 2, false, LONG>(ma, mb, a, tiles, 1, s);
-    const bool split = shape.ranks > 1;
-    if (shape.bn == 32)
-        return split ? gl_launch<MODE, kNarrowest, 1, true, LONG>(ma, mb, a, tiles, shape.ranks, s)
-                     : gl_launch<MODE, kNarrowest, 1, false, LONG>(ma, mb, a, tiles, 1, s);
-    if (shape.bn == 64)
-        return split ? gl_launch<MODE, 64, 1, true, LONG>(ma, mb, a, tiles, shape.ranks, s)
-                     : gl_launch<MODE, 64, 1, false, LONG>(ma, mb, a, tiles, 1, s);
-    if (shape.bn == 128)
-        return split ? gl_launch<MODE, 128, 1, true, LONG>(ma, mb, a, tiles, shape.ranks, s)
-                     : gl_launch<MODE, 128, 1, false, LONG>(ma, mb, a, tiles, 1, s);
-    return split ? gl_launch<MODE, kWidest, 1, true, LONG>(ma, mb, a, tiles, shape.ranks, s)
-                 : gl_launch<MODE, kWidest, 1, false, LONG>(ma, mb, a, tiles, 1, s);
+    if (shape.ranks > 1) return gl_launch<MODE, kNarrowest, 1, true, LONG>(ma, mb, a, tiles, shape.ranks, s);
+    if (shape.bn == 32) return gl_launch<MODE, kNarrowest, 1, false, LONG>(ma, mb, a, tiles, 1, s);
+    if (shape.bn == 64) return gl_launch<MODE, 64, 1, false, LONG>(ma, mb, a, tiles, 1, s);
+    if (shape.bn == 128) return gl_launch<MODE, 128, 1, false, LONG>(ma, mb, a, tiles, 1, s);
+    return gl_launch<MODE, kWidest, 1, false, LONG>(ma, mb, a, tiles, 1, s);
 }
 
 static CUtensorMapDataType map_type(int32_t type) {

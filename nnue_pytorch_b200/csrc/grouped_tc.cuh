@@ -34,8 +34,8 @@ inline TileShape tile_shape(int64_t runs, int64_t rows, int64_t cols, int64_t ch
     if (pairs && rows > kGroupRows && tiles(kGroupPairRows, widest) * 2 >= sms) return {widest, 2, 1};
     int bn = widest;
     while (bn > narrowest && (tiles(kGroupRows, bn) < sms || cols <= bn / 2)) bn /= 2;
-    int ranks = 1;
-    while (ranks < 8 && tiles(kGroupRows, bn) * ranks * 2 <= sms && chunks >= ranks * 4) ranks *= 2;
+    int ranks = 1;  // more only at the narrowest: a wider tile was kept because every SM has one
+    while (bn == narrowest && ranks < 8 && tiles(kGroupRows, bn) * ranks * 2 <= sms && chunks >= ranks * 4) ranks *= 2;
     return {bn, 1, ranks};
 }
 
