@@ -769,7 +769,8 @@ int nnue_group_sums(const float* sums, const void* plan, void* out,
  * bwd_weight takes both laid out, and dy's sums where dbias is wanted.
  * bias [E, N] of any of the three float types, may be NULL; y [T, N], dx [T, K] and
  * dw [E, N, K] contiguous, y and dw of `type` or F32, dx of `type`, dbias [E, N] of
- * any float type, may be NULL.  Sums are fp32, rounded once.  Rows without a
+ * any float type, may be NULL.  Sums are fp32 (runs of 512 terms by the tensor core,
+ * whose additions cut off, and the runs added rounding to nearest), rounded once.  Rows without a
  * bucket get zeros in y and dx, whatever they hold; a bucket without rows gets
  * zeros in dw and dbias.  Sums run in an order that the sizes alone fix: results
  * are reproducible.  T = 0 is allowed.  `plan`: nnue_group_plan's, of the same T

@@ -238,29 +238,7 @@ __device__ __forceinline__ void f8_bring_out(const F8Args& a, const F8Tile& x, f
         }
         __syncwarp();
     }
-    if (a.o.type == NNUE_T_F32) {
-#pragma unroll
-        for (int h = 0; h < HALF; h += 32) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p)
-                *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
-                    make_float4(acc[h + 4 * p], acc[h + 4 * p + 1], acc[h + 4 * p + 2], acc[h + 4 * p + 3]);
-            copy_rows_out<128>(a.o, stg, my_row, 0, col + h);
-        }
-    } else {
-        constexpr int kPass = HALF < 64 ? HALF : 64;
-#pragma unroll
-        for (int h = 0; h < HALF; h += kPass) {
-#pragma unroll
-            for (int p = 0; p < kPass / 8; ++p) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = pack_half(acc[h + 8 * p + 2 * j], acc[h + 8 * p + 2 * j + 1], a.o.type);
-                *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            copy_rows_out<kPass * 2>(a.o, stg, my_row, 0, col + h);
-        }
-    }
+    bring_out<0, HALF>(a.o, acc, stg, my_row, 0, col);
 }
 
 template <int BN, int CTAS, bool SPLIT>

@@ -14,19 +14,25 @@
 // 4096 x 2048), and rows gathered by 16-byte asynchronous copies came to 36 GB/s per SM with four warps (254 us; 595 for
 // dw): laying the rows out first costs 42 us there, and both directions read them.
 //
-// Roles: warp 0 copies into a ring of stages, warp 1 issues the instructions, warps 2-9 bring finished
-// tiles out while the next tile multiplies (two accumulators).  Persistent: a CTA (or pair) per SM walks the tiles with
-// a stride of the grid.
+// Roles: warp 0 copies into a ring of stages, warp 1 issues the instructions, warps 4-11 take the accumulators and bring
+// finished tiles out while the next run of stages multiplies (two accumulators).  Persistent: a CTA (or pair) per SM walks
+// the tiles with a stride of the grid.
 // CTAS = 2: a pair of SMs works on 256 rows x BN columns, each holding its half of A and of B: half the bytes of B per
 //   SM and flop, through L2 and in shared memory, which is what bounds a single CTA (96 bytes per cycle wanted of L2's
 //   64 at 128 x 256).
 // SPLIT: few tiles; a cluster of 2 to 8 CTAs splits the sum, the partial tiles meet in distributed shared memory and are
 //   added in the order of the ranks.
-// LONG (dw in fp32): the tensor core's adder cuts off, so an error grows with the number of additions (2.4e-6 of the
-//   gradient at 2048 rows).  Every 512 rows the accumulator is added, rounding to nearest, to a total that also lives in
-//   tensor memory.
-// Measured at 16384 x 4096 x 2048 over 8 buckets, bf16: forward 180 us (1.53 PFLOP/s), dx 198, dw 226 after 41 us for laying
-//   x out and 20 for dy; the operands' way through L2 and shared memory bounds all three (32 KB per SM and stage).
+// Sums in two levels: the tensor core's adder cuts off.  Measured on sums next to 2^23: each of an instruction's 16 terms
+//   loses what lies below a quarter of the sum's last bit, the result what lies below that bit, so an addition loses
+//   less than 5 x 2^-23 of the sum and a sum of n terms grows off by n / 16 times that.  An accumulator therefore adds up runs
+//   of 512 terms; the output warps hold the sums in registers (half a row of the tile per thread) and add the runs rounding
+//   to nearest.  In one level the sums of 16384 x 4096 x 2048 came out 9 times as far off as those of an fp32 product.
+//   Runs of 8 stages against one for the whole sum, us at that size over 8 buckets: forward 198 (183), dx 202 (197), dw 221
+//   (219); of 4 stages 213, 212, 221; of 16 193, 198, 218: a change of accumulator costs the issuing warp about 400
+//   cycles.  dw in fp32 227 (353 with the total in tensor memory, which leaves room for 128 columns only).
+// Measured at that size, bf16: forward 198 us (1.39 PFLOP/s), dx 202, dw 221 after 81 for laying x and dy out; bound by the
+// issuing warp's way from stage to stage (about 800 cycles for 512 of multiplying) and the operands' way through L2 and
+// shared memory (32 KB per SM and stage).
 // All orders are fixed by the sizes: results are reproducible.  Every wait is bounded; one that runs out raises the
 // device status word and the CTA leaves, its tensor memory freed; copies in flight are then as old as that wait.
 #include "grouped_tc.cuh"
@@ -38,8 +44,13 @@ enum { kModeFwd = 0, kModeDx = 1, kModeDw = 2 };
 constexpr int kGlK = 64;                     // reduction elements per stage: one 128-byte swizzle row
 constexpr int kGlABytes = kGroupRows * 128;  // 16 KiB
 constexpr int kGlBoxBytes = kGlK * 128;      // MN-major block: 64 rows of the reduction x 128 bytes
-constexpr int kGlThreads = 320;
-constexpr int kGlLong = 8;                   // stages between additions to the total
+constexpr int kGlThreads = 384;  // copies, instructions, two warps without work, eight output warps
+constexpr int kGlOutWarp = 4;    // the first output warp
+// An output thread of the widest tile holds 128 sums and two reads of 32 columns: the first warpgroup gives registers up
+// (at 72 and 216 the sums spill: dx 210 us for 202).
+constexpr int kGlFewRegs = 56, kGlManyRegs = 224, kGlLaunchRegs = 168;
+static_assert(128 * kGlFewRegs + 256 * kGlManyRegs <= kGlThreads * kGlLaunchRegs, "more registers than the launch brings");
+constexpr int kGlRun = 8;                    // stages that one accumulator adds up: 512 terms
 
 constexpr int gl_stage_bytes(int bn, int ctas) { return kGlABytes + bn / ctas * 128; }
 constexpr int gl_stages(int bn, int ctas) { return gl_stage_bytes(bn, ctas) > 32768 ? 4 : gl_stage_bytes(bn, ctas) > 24576 ? 6 : 8; }
@@ -108,79 +119,35 @@ __device__ __forceinline__ int gl_steps(const GlArgs& a, const GlTile& x, int c)
     return left >= kGlK ? 4 : (left + 15) >> 4;
 }
 
-// One output warp: its 32 rows and COLS columns of the tile, from tensor memory (or zeros) to the output.  `bias`: where the
-// warp's first column's is, or null.
-template <int COLS>
-__device__ __forceinline__ void gl_bring_out(const GlArgs& a, uint32_t taddr, bool zeros, bool biased, int64_t bias_at, unsigned char* stg,
-                                             int32_t my_row, int64_t row_base, int col0) {
-    const int lane = threadIdx.x & 31;
-    const bool f32 = a.o.type == NNUE_T_F32;
-    const bool wide = !f32 && COLS >= 64;  // two reads of 32 columns make one 128-byte piece of a row
-    const int step = wide ? 64 : 32;
-    float* s_bias = reinterpret_cast<float*>(stg);
-    float next[2] = {0.f, 0.f};  // bias of the next columns, on its way while these go out
-    auto fetch = [&](int c) {
+// a0 += v0, a1 += v1, each rounded to nearest
+__device__ __forceinline__ void add2(float& a0, float& a1, uint32_t v0, uint32_t v1) {
+    unsigned long long a, v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(v));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
+}
+
+// One output warp: sum (FIRST: =, else +=, rounding to nearest) accumulator, its 32 lanes and COLS columns.
+template <int COLS, bool FIRST>
+__device__ __forceinline__ void gl_add(uint32_t taddr, float (&sum)[COLS]) {
+    constexpr int kReads = COLS / 32, kAtOnce = kReads < 2 ? kReads : 2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int j = c + 32 * h + lane;
-            next[h] = 32 * h < step && j < COLS && col0 + j < a.o.cols ? load_as_float(a.bias, a.bias_type, bias_at + j) : 0.f;
-        }
-    };
-    if (biased) fetch(0);
-#pragma unroll 1
-    for (int c = 0; c < COLS && col0 + c < a.o.cols; c += step) {
-        if (biased) {
-            s_bias[lane] = next[0];
-            s_bias[32 + lane] = next[1];
-            fetch(c + step);
-            __syncwarp();
-        }
-        uint32_t v[2][32];
-        if (zeros) {
+    for (int c = 0; c < kReads; c += kAtOnce) {
+        uint32_t v[kAtOnce][32];  // the reads under way before the wait
 #pragma unroll
-            for (int j = 0; j < 64; ++j) v[j / 32][j % 32] = 0u;
-        } else {  // both reads under way before the wait
-            tmem_ld32(taddr + c, v[0]);
-            if (wide) tmem_ld32(taddr + c + 32, v[1]);
-            tmem_wait_ld(v[0]);
-            if (wide) tmem_wait_ld(v[1]);
-        }
-        if (biased) {
+        for (int h = 0; h < kAtOnce; ++h) tmem_ld32(taddr + 32 * (c + h), v[h]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h == 1 && !wide) break;
+        for (int h = 0; h < kAtOnce; ++h) tmem_wait_ld(v[h]);
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 b = *reinterpret_cast<const float4*>(s_bias + 32 * h + j);
-                    v[h][j] = __float_as_uint(__uint_as_float(v[h][j]) + b.x);
-                    v[h][j + 1] = __float_as_uint(__uint_as_float(v[h][j + 1]) + b.y);
-                    v[h][j + 2] = __float_as_uint(__uint_as_float(v[h][j + 2]) + b.z);
-                    v[h][j + 3] = __float_as_uint(__uint_as_float(v[h][j + 3]) + b.w);
-                }
+        for (int h = 0; h < kAtOnce; ++h)
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                float& s0 = sum[32 * (c + h) + j];
+                float& s1 = sum[32 * (c + h) + j + 1];
+                if (FIRST) s0 = __uint_as_float(v[h][j]), s1 = __uint_as_float(v[h][j + 1]);
+                else add2(s0, s1, v[h][j], v[h][j + 1]);
             }
-            __syncwarp();
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (h == 1 && !wide) break;
-            if (f32) {
-#pragma unroll
-                for (int p = 0; p < 8; ++p)
-                    *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) =
-                        make_uint4(v[h][4 * p], v[h][4 * p + 1], v[h][4 * p + 2], v[h][4 * p + 3]);
-            } else {
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        w[j] = pack_half(__uint_as_float(v[h][8 * p + 2 * j]), __uint_as_float(v[h][8 * p + 2 * j + 1]), a.o.type);
-                    *reinterpret_cast<uint4*>(stg + lane * 128 + (((4 * h + p) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-        }
-        if (f32 || wide) copy_rows_out<128>(a.o, stg, my_row, row_base, col0 + c);
-        else copy_rows_out<64>(a.o, stg, my_row, row_base, col0 + c);
     }
 }
 
@@ -247,7 +214,7 @@ __device__ __forceinline__ bool gl_copy_role(const GlArgs& a, const CUtensorMap*
 }
 
 // ---- warp 1: the instructions -------------------------------------------------------------------------------------
-template <int MODE, int BN, int CTAS, bool SPLIT, bool LONG>
+template <int MODE, int BN, int CTAS, bool SPLIT>
 __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, uint32_t ring, uint64_t* full, uint64_t* empty,
                                               uint64_t* done, uint64_t* taken, uint64_t* drained, int t0, int stride, int tiles,
                                               int rank, int ranks) {
@@ -259,8 +226,8 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
     bool ok = true;
     for (int t = t0; t < tiles && ok; t += stride) {
         const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
-        for (int g = x.c0; g < x.c1 && ok; g += LONG ? kGlLong : x.c1 - x.c0) {  // one accumulator's chunks
-            const int end = LONG ? min(x.c1, g + kGlLong) : x.c1;
+        for (int g = x.c0; g < x.c1 && ok; g += kGlRun) {  // one accumulator's chunks
+            const int end = min(x.c1, g + kGlRun);
             ok = mbar_wait_warp(taken + acc.stage, acc.phase ^ 1u);
             if (!ok) break;
             tc_fence_after();
@@ -294,27 +261,6 @@ __device__ __forceinline__ bool gl_issue_role(const GlArgs& a, uint32_t tmem, ui
     return ok;
 }
 
-// One output warp: total (+)= accumulator, its 32 lanes.
-template <int COLS>
-__device__ __forceinline__ void gl_add_to_total(uint32_t acc, uint32_t total, bool first) {
-#pragma unroll 1
-    for (int c = 0; c < COLS; c += 32) {
-        uint32_t v[32], w[32];
-        tmem_ld32(acc + c, v);
-        if (!first) {
-            tmem_ld32(total + c, w);
-            tmem_wait_ld(v);
-            tmem_wait_ld(w);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
-        } else {
-            tmem_wait_ld(v);
-        }
-        tmem_st32(total + c, v);
-    }
-    tmem_wait_st();
-}
-
 // dw: dbias of this thread's row, from the sums of the bucket's tiles in order
 __device__ __forceinline__ void gl_bias_gradient(const GlArgs& a, const GlTile& x, int n) {
     float total = 0.f;
@@ -324,14 +270,14 @@ __device__ __forceinline__ void gl_bias_gradient(const GlArgs& a, const GlTile& 
     store_from_float(a.sums, a.sums_type, (int64_t)x.bucket * a.N + n, total);
 }
 
-template <int MODE, int BN, int CTAS, bool SPLIT, bool LONG>
+template <int MODE, int BN, int CTAS, bool SPLIT>
 __global__ void __launch_bounds__(kGlThreads, 1)
     k_grouped(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GlArgs a) {
     constexpr bool PAIR = CTAS == 2;
     constexpr int S = gl_stages(BN, CTAS);
-    constexpr uint32_t kTmemCols = LONG && 3 * BN > 256 ? 512 : LONG ? 4 * BN : 2 * BN;
+    constexpr uint32_t kTmemCols = 2 * BN;
     constexpr int kPartPitch = BN + 4;  // floats per row of a partial tile
-    static_assert(!(PAIR && SPLIT) && (!LONG || (MODE == kModeDw && BN <= 128)), "no such variant");
+    static_assert(!(PAIR && SPLIT), "no such variant");
     extern __shared__ unsigned char smem_raw[];
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* ring_ptr = smem_raw + (ring - smem_u32(smem_raw));
@@ -377,20 +323,21 @@ __global__ void __launch_bounds__(kGlThreads, 1)
     const uint32_t tmem = *s_tmem;
 
     bool ok = true;
-    if (warp == 0) {
-        ok = gl_copy_role<MODE, BN, CTAS, SPLIT>(a, &map_a, &map_b, ring, full, empty, t0, stride, tiles, rank, ranks);
-    } else if (warp == 1) {
-        if (!(PAIR && rank != 0))
-            ok = gl_issue_role<MODE, BN, CTAS, SPLIT, LONG>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
+    if (warp < kGlOutWarp) {
+        if (BN == 256) fewer_registers<kGlFewRegs>();
+        if (warp == 0)
+            ok = gl_copy_role<MODE, BN, CTAS, SPLIT>(a, &map_a, &map_b, ring, full, empty, t0, stride, tiles, rank, ranks);
+        else if (warp == 1 && !(PAIR && rank != 0))
+            ok = gl_issue_role<MODE, BN, CTAS, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
     } else {
+        if (BN == 256) more_registers<kGlManyRegs>();
         constexpr int kCols = gl_warp_cols(BN);
-        const int q = warp & 3, half = (warp - 2) >> 2;  // the quarter of tensor memory's lanes, the half of the columns
-        const bool works = half * kCols < BN;            // 32 columns are one half
+        const int q = warp & 3, half = (warp - kGlOutWarp) >> 2;  // the quarter of tensor memory's lanes, the half of the columns
+        const bool works = BN >= 64 || half == 0;                 // 32 columns are one half
         const uint32_t lanes = ((uint32_t)(q * 32) << 16) + half * kCols;
         StageRing<2> acc;
         for (int t = t0; t < tiles && ok; t += stride) {
             const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t, rank, ranks);
-            const bool some = x.c1 > x.c0;
             const int r = (PAIR ? rank * kGroupRows : 0) + q * 32 + lane;
             int32_t my_row;
             int64_t row_base = 0;
@@ -401,8 +348,18 @@ __global__ void __launch_bounds__(kGlThreads, 1)
             } else {
                 my_row = r < x.count ? __ldg(a.plan.order + x.first + r) : -1;
             }
+            const int col = x.col0 + half * kCols;
             const bool biased = MODE == kModeFwd && !SPLIT && a.bias && x.live;
-            auto give_back = [&] {
+            float bias[kCols / 32];  // of columns lane, 32 + lane, ..: on its way while the tile multiplies
+            if (biased) {
+#pragma unroll
+                for (int i = 0; i < kCols / 32; ++i) {
+                    const int j = 32 * i + lane;
+                    bias[i] = works && col + j < a.o.cols ? load_as_float(a.bias, a.bias_type, (int64_t)x.bucket * a.N + col + j) : 0.f;
+                }
+            }
+            float sum[kCols];
+            auto taken_in = [&] {  // the accumulator is in registers
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -411,52 +368,59 @@ __global__ void __launch_bounds__(kGlThreads, 1)
                 }
                 acc.next();
             };
-            uint32_t from = tmem + lanes + acc.stage * BN;
-            if (LONG) {
-                for (int g = x.c0; g < x.c1; g += kGlLong) {
+            if (x.c0 < x.c1) {
+                ok = mbar_wait_warp(done + acc.stage, acc.phase);
+                if (!ok) break;
+                tc_fence_after();
+                if (works) gl_add<kCols, true>(tmem + lanes + acc.stage * BN, sum);
+                taken_in();
+#pragma unroll 1
+                for (int g = x.c0 + kGlRun; g < x.c1; g += kGlRun) {
                     ok = mbar_wait_warp(done + acc.stage, acc.phase);
                     if (!ok) break;
                     tc_fence_after();
-                    if (works) gl_add_to_total<kCols>(tmem + lanes + acc.stage * BN, tmem + lanes + 2 * BN, g == x.c0);
-                    give_back();
+                    if (works) gl_add<kCols, false>(tmem + lanes + acc.stage * BN, sum);
+                    taken_in();
                 }
-                from = tmem + lanes + 2 * BN;
-            } else if (some) {
-                ok = mbar_wait_warp(done + acc.stage, acc.phase);
-                if (ok) tc_fence_after();
+                if (!ok) break;
+            } else {
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sum[j] = 0.f;
             }
-            if (!ok || SPLIT) break;
-            const int col = x.col0 + half * kCols;
-            if (works && __any_sync(kFullMask, my_row >= 0))
-                gl_bring_out<kCols>(a, from, !some, biased && some, (int64_t)x.bucket * a.N + col, staging + (warp - 2) * kStagingBytes, my_row,
-                                    row_base, col);
-            if (!LONG && some) give_back();
+            if (SPLIT) {
+                // the last accumulator is complete, so nothing reads the ring any more: it takes the partial tile
+                float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * kPartPitch + half * kCols;
+                if (works) {
+#pragma unroll
+                    for (int j = 0; j < kCols; j += 4) *reinterpret_cast<float4*>(part + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+                }
+                break;
+            }
+            if (!works || col >= a.o.cols || !__any_sync(kFullMask, my_row >= 0)) continue;
+            unsigned char* stg = staging + (warp - kGlOutWarp) * kStagingBytes;
+            if (biased) {
+                float* s_bias = reinterpret_cast<float*>(stg);
+#pragma unroll
+                for (int i = 0; i < kCols / 32; ++i) s_bias[32 * i + lane] = bias[i];
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < kCols; j += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(s_bias + j);
+                    sum[j] += b.x;
+                    sum[j + 1] += b.y;
+                    sum[j + 2] += b.z;
+                    sum[j + 3] += b.w;
+                }
+                __syncwarp();
+            }
+            bring_out<0, kCols>(a.o, sum, stg, my_row, row_base, col);
         }
     }
     __syncwarp();
     if (!ok && lane == 0) note_timeout(a.status);
 
     if (SPLIT) {
-        __syncthreads();  // nobody reads the ring any more: the partial tile takes its place
         const GlTile x = gl_tile<MODE, BN, CTAS, SPLIT>(a, t0, rank, ranks);
-        if (warp >= 2) {
-            const int q = warp & 3, half = (warp - 2) >> 2;
-            float* part = reinterpret_cast<float*>(ring_ptr) + (q * 32 + lane) * kPartPitch;
-#pragma unroll 1
-            for (int c = half * gl_warp_cols(BN); c < min(BN, (half + 1) * gl_warp_cols(BN)); c += 32) {
-                uint32_t v[32];
-                if (x.c1 > x.c0) {
-                    tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (LONG ? 2 * BN : 0) + c, v);
-                    tmem_wait_ld(v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0u;
-                }
-#pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    *reinterpret_cast<uint4*>(part + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            }
-        }
         cluster_sync();
         // row r of the tile is finished by rank r mod ranks: partial sums in the order of the ranks
         const int rows = MODE == kModeDw ? min(kGroupRows, a.N - x.row0) : x.count;
@@ -504,14 +468,18 @@ __global__ void __launch_bounds__(kGlThreads, 1)
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
-template <int MODE, int BN, int CTAS, bool SPLIT, bool LONG>
+template <int MODE, int BN, int CTAS, bool SPLIT>
 int gl_launch(const CUtensorMap& ma, const CUtensorMap& mb, const GlArgs& a, int64_t tiles, int ranks, cudaStream_t s) {
-    auto kernel = k_grouped<MODE, BN, CTAS, SPLIT, LONG>;
+    auto kernel = k_grouped<MODE, BN, CTAS, SPLIT>;
     static bool opted[64] = {};  // more than 48 KB of dynamic shared memory needs the opt-in, once per device
     int dev = 0;
     NNUE_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !opted[dev]) {
         NNUE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gl_smem(BN, CTAS)));
+        cudaFuncAttributes attr;
+        NNUE_CUDA_TRY(cudaFuncGetAttributes(&attr, kernel));
+        NNUE_REQUIRE(BN != 256 || attr.numRegs >= kGlLaunchRegs, NNUE_ERR_UNSUPPORTED, "grouped linear: built with %d registers per thread",
+                     attr.numRegs);
         if (dev >= 0 && dev < 64) opted[dev] = true;
     }
     const int64_t at_once = sm_count() / CTAS;
@@ -534,19 +502,19 @@ int gl_launch(const CUtensorMap& ma, const CUtensorMap& mb, const GlArgs& a, int
     return NNUE_OK;
 }
 
-template <int MODE, bool LONG>
+template <int MODE>
 int gl_run(const CUtensorMap& ma, const CUtensorMap& mb, GlArgs& a, int64_t tile_rows, TileShape shape, cudaStream_t s) {
-    constexpr int kNarrowest = MODE == kModeFwd ? 32 : 64, kWidest = LONG ? 128 : 256;
+    constexpr int kNarrowest = MODE == kModeFwd ? 32 : 64, kWidest = 256;
     a.col_tiles = (a.o.cols + shape.bn - 1) / shape.bn;
     a.idesc = umma_idesc(a.idesc, (uint32_t)(kGroupRows * shape.ctas), (uint32_t)shape.bn, MODE == kModeDw, MODE != kModeFwd);
     const int64_t tiles = tile_rows * a.col_tiles;
     NNUE_REQUIRE(tiles * 8 < 0x7fffffffLL, NNUE_ERR_UNSUPPORTED, "grouped linear: too many tiles");
-    if (shape.ctas == 2) return gl_launch<MODE, kWidest, 2, false, LONG>(ma, mb, a, tiles, 1, s);
-    if (shape.ranks > 1) return gl_launch<MODE, kNarrowest, 1, true, LONG>(ma, mb, a, tiles, shape.ranks, s);
-    if (shape.bn == 32) return gl_launch<MODE, kNarrowest, 1, false, LONG>(ma, mb, a, tiles, 1, s);
-    if (shape.bn == 64) return gl_launch<MODE, 64, 1, false, LONG>(ma, mb, a, tiles, 1, s);
-    if (shape.bn == 128) return gl_launch<MODE, 128, 1, false, LONG>(ma, mb, a, tiles, 1, s);
-    return gl_launch<MODE, kWidest, 1, false, LONG>(ma, mb, a, tiles, 1, s);
+    if (shape.ctas == 2) return gl_launch<MODE, kWidest, 2, false>(ma, mb, a, tiles, 1, s);
+    if (shape.ranks > 1) return gl_launch<MODE, kNarrowest, 1, true>(ma, mb, a, tiles, shape.ranks, s);
+    if (shape.bn == 32) return gl_launch<MODE, kNarrowest, 1, false>(ma, mb, a, tiles, 1, s);
+    if (shape.bn == 64) return gl_launch<MODE, 64, 1, false>(ma, mb, a, tiles, 1, s);
+    if (shape.bn == 128) return gl_launch<MODE, 128, 1, false>(ma, mb, a, tiles, 1, s);
+    return gl_launch<MODE, kWidest, 1, false>(ma, mb, a, tiles, 1, s);
 }
 
 static CUtensorMapDataType map_type(int32_t type) {
@@ -630,7 +598,7 @@ extern "C" int nnue_grouped_linear_fwd(const void* x, int64_t ldx, int32_t laid,
     CUtensorMap ma, mb;
     if (int st = operand_map(&ma, &a, laid, x, ldx, T, K, E, type)) return st;
     if (int st = weight_map(&mb, w, ldw, E, N, K, shape.bn / shape.ctas, type)) return st;
-    return gl_run<kModeFwd, false>(ma, mb, a, group_max_tiles(T, E), shape, s);
+    return gl_run<kModeFwd>(ma, mb, a, group_max_tiles(T, E), shape, s);
 }
 
 extern "C" int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, int32_t laid, const void* w, int64_t ldw, const void* plan,
@@ -651,7 +619,7 @@ extern "C" int nnue_grouped_linear_bwd_input(const void* dy, int64_t lddy, int32
     CUtensorMap ma, mb;
     if (int st = operand_map(&ma, &a, laid, dy, lddy, T, N, E, type)) return st;
     if (int st = weight_map(&mb, w, ldw, E, N, K, 64, type)) return st;
-    return gl_run<kModeDx, false>(ma, mb, a, group_max_tiles(T, E), shape, s);
+    return gl_run<kModeDx>(ma, mb, a, group_max_tiles(T, E), shape, s);
 }
 
 extern "C" int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_sums, const void* x, const void* plan, void* dw,
@@ -674,9 +642,8 @@ extern "C" int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_su
     a.tile_sums = dy_sums;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     ProfScope prof("grouped_dw", s);
-    const bool fp32 = dw_type == NNUE_T_F32;
     const int64_t mean = (T + E - 1) / E;
-    const TileShape shape = tile_shape(E, N, K, (mean + kGlK - 1) / kGlK, 64, fp32 ? 128 : 256, true);
+    const TileShape shape = tile_shape(E, N, K, (mean + kGlK - 1) / kGlK, 64, 256, true);
     a.row_tiles = (int32_t)((N + kGroupRows * shape.ctas - 1) / (kGroupRows * shape.ctas));
     CUtensorMap ma, mb;
     if (T > 0) {
@@ -686,6 +653,5 @@ extern "C" int nnue_grouped_linear_bwd_weight(const void* dy, const float* dy_su
         if (int st = rows_map(&ma, dw, 64, 1, 1, 1, type)) return st;
         mb = ma;
     }
-    return fp32 ? gl_run<kModeDw, true>(ma, mb, a, (int64_t)E * a.row_tiles, shape, s)
-                : gl_run<kModeDw, false>(ma, mb, a, (int64_t)E * a.row_tiles, shape, s);
+    return gl_run<kModeDw>(ma, mb, a, (int64_t)E * a.row_tiles, shape, s);
 }

@@ -103,6 +103,39 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b, int32_t type) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// An output warp's 32 rows and the sums [FROM, FROM + COUNT) of each, to the output from column `col` on: one rounding.
+template <int FROM, int COUNT, int COLS>
+__device__ __forceinline__ void bring_out(const RowsOut& o, const float (&sum)[COLS], unsigned char* stg, int32_t my_row, int64_t row_base,
+                                          int col) {
+    const int lane = threadIdx.x & 31;
+    if (o.type == NNUE_T_F32) {
+#pragma unroll
+        for (int h = 0; h < COUNT; h += 32) {
+            if (col + h >= o.cols) break;
+            const float* v = sum + FROM + h;
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                *reinterpret_cast<float4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+            copy_rows_out<128>(o, stg, my_row, row_base, col + h);
+        }
+    } else {
+        constexpr int kPass = COUNT < 64 ? COUNT : 64;
+#pragma unroll
+        for (int h = 0; h < COUNT; h += kPass) {
+            if (col + h >= o.cols) break;
+            const float* v = sum + FROM + h;
+#pragma unroll
+            for (int p = 0; p < kPass / 8; ++p) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = pack_half(v[8 * p + 2 * j], v[8 * p + 2 * j + 1], o.type);
+                *reinterpret_cast<uint4*>(stg + lane * 128 + ((p ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            copy_rows_out<kPass * 2>(o, stg, my_row, row_base, col + h);
+        }
+    }
+}
+
 #endif  // __CUDACC__
 
 }  // namespace nnue

@@ -38,3 +38,70 @@ def test_saved_tensors_kept_on_the_host(dev, T):
         close(x.grad, *ref["dx"], "dx")
         if train_weights:
             close(w.grad, *ref["dw"], "dw")
+
+
+# ---- accuracy of long sums.  One addition of the tensor core takes 16 terms: each loses what lies below a quarter of the
+# last bit of the largest, their sum what lies below its own last bit, together less than 5 * 2^-23 of the sum.  A run of 512
+# terms of one sign is 32 additions to partial sums that are no larger than the run.  Runs are added rounding to nearest, at
+# most 2^-24 of the sum each, and where a sum is split over ranks, up to 8 additions more.
+def _long_sum_bound(terms):
+    return 32 * 5 * 2.0**-23 + (-(-terms // 512) + 8) * 2.0**-24
+
+
+def _near(ours, ref, terms, what):
+    bound = ref.abs() * _long_sum_bound(terms)
+    if ours.dtype != torch.float32:
+        bound += (ref.abs() + bound) * (torch.finfo(ours.dtype).eps / 2)
+    off = (ours.double() - ref).abs()
+    assert (off <= bound).all(), f"{what}: off by {float((off / ref.abs()).max()):.3e} of the sum, allowed {float((bound / ref.abs()).max()):.3e}"
+
+
+def _one_sign(g, dev, *shape):
+    return (torch.rand(*shape, generator=g, device=dev) * 0.5 + 0.25).bfloat16()
+
+
+@pytest.mark.parametrize("T,K,N", [(60, 16384, 40), (300, 16384, 1000), (2500, 8192, 2100), (20000, 8192, 200)])
+def test_long_sums_of_the_forward_in_fp32(dev, T, K, N):
+    """One, several and all-SM tiles, single CTAs and pairs."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator(device=dev).manual_seed(51)
+    x, w = _one_sign(g, dev, T, K), _one_sign(g, dev, N, K)
+    plan = GroupPlan(torch.zeros(T, dtype=torch.int64, device=dev), 1)
+    _near(grouped_linear(x, w, None, plan, out_dtype=torch.float32), x.double() @ w.double().T, K, "y")
+
+
+@pytest.mark.parametrize("K,N", [(64, 40), (2048, 200), (1280, 2100)])  # split sums, single CTAs, pairs
+def test_long_sums_of_the_weight_gradient_in_fp32(dev, K, N):
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    T = 16000
+    g = torch.Generator(device=dev).manual_seed(52)
+    x, dy = _one_sign(g, dev, T, K), _one_sign(g, dev, T, N)
+    w = torch.zeros(N, K, device=dev, requires_grad=True)
+    y = grouped_linear(x, w, None, GroupPlan(torch.zeros(T, dtype=torch.int64, device=dev), 1))
+    dw, = torch.autograd.grad(y, w, dy)
+    _near(dw, dy.double().T @ x.double(), T, "dw")
+
+
+@pytest.mark.parametrize("direction", ["y", "dx", "dw"])
+def test_very_long_sums_in_16_bits(dev, direction):
+    """2^20 terms: what is cut off may not outgrow the one rounding to fp16."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator(device=dev).manual_seed(53)
+    long, T, K, N = 1 << 20, 48, 16, 24
+    T, K, N = {"y": (T, long, N), "dx": (T, K, long), "dw": (long, K, N)}[direction]
+    small = 2.0**-8  # 2^20 products near 1/4 stay within fp16
+    x, w, dy = ((_one_sign(g, dev, *s) * small).half().requires_grad_(True) for s in ((T, K), (N, K), (T, N)))
+    if direction == "y":
+        y = grouped_linear(x.detach(), w.detach() / small, None, GroupPlan(torch.zeros(T, dtype=torch.int64, device=dev), 1))
+        _near(y, x.detach().double() @ (w.detach() / small).double().T, long, "y")
+        return
+    y = grouped_linear(x, w, None, GroupPlan(torch.zeros(T, dtype=torch.int64, device=dev), 1))
+    if direction == "dx":
+        dx, = torch.autograd.grad(y, x, dy.detach() / small)
+        _near(dx, (dy.detach() / small).double() @ w.detach().double(), long, "dx")
+    else:
+        dw, = torch.autograd.grad(y, w, dy.detach() / small)
+        _near(dw, (dy.detach() / small).double().T @ x.detach().double(), long, "dw")
