@@ -9,12 +9,15 @@
 // Bound by the way of an accumulator, not by the tensor core: a stage of a pair of SMs on 256 x 256 multiplies in 390 cycles,
 // but its first result is there after 900, is read and scaled in 700 to 900 and given back in 240, and tensor memory holds
 // two: about 1000 cycles per stage (16384 x 4096 x 2048 over 8 buckets: 175 us, 1.57 PFLOP/s; 135 us of it are stages at
-// work, 20 to 40 the bringing out of eight tiles per pair).  Four accumulators of 128 columns halve the way but double the stages
+// work, 20 to 40 the bringing out of eight tiles per pair; 180 with the test of the scales below).  Four accumulators of 128 columns halve the way but double the stages
 // (223 us), and two products of 128 columns per stage came to 219.
 // Copies, pairs of SMs, split sums and bounded waits as in the 16-bit kernel (grouped_linear.cu).  Rows come laid out by
 // bucket (the quantiser leaves them so), in their own order where there is one matrix, or are gathered by TMA, four per
 // copy, where a bucket has few.
 #include "grouped_tc.cuh"
+
+#include <type_traits>
+
 namespace nnue {
 
 constexpr int kF8K = 128;
@@ -163,10 +166,17 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t v0, uint32_t
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
 }
 
+// A block's sum is multiplied by sx * sw at once where that product is a normal number.  Else an output warp multiplies by the
+// larger scale first: what comes out in range then meets neither an overflow nor a loss of digits on the way (the smaller
+// one only takes it down where the product is too small, up where it is too large).  A second loop does that from the first
+// such group of a tile on: the first loop pays one test per group (16384 x 4096 x 2048 over 8 buckets: 180 us for 175;
+// with the test in every stage of one loop 213).
+__device__ __forceinline__ bool is_normal(float p) { return fabsf(p) >= 1.17549435e-38f && fabsf(p) <= 3.40282347e38f; }
+
 // One warp: sx * sw of every row and half of the columns, four stages at a time, into the ring that the output warps read.
 // (As loads of the output warps themselves they were waited for in every stage: their registers hold the sums.)
 template <int BN, int CTAS, bool SPLIT>
-__device__ __forceinline__ bool f8_scale_role(const F8Args& a, float* slots, uint64_t* sfull, uint64_t* sfree, int t0, int stride,
+__device__ __forceinline__ bool f8_scale_role(const F8Args& a, float* slots, int* apart, uint64_t* sfull, uint64_t* sfree, int t0, int stride,
                                               int tiles, int rank, int ranks) {
     constexpr int kHalves = f8_slot_floats(BN) / kGroupRows;
     const int lane = threadIdx.x & 31, r0 = 4 * lane + (CTAS == 2 ? rank * kGroupRows : 0);
@@ -198,19 +208,25 @@ __device__ __forceinline__ bool f8_scale_role(const F8Args& a, float* slots, uin
                     v[i][3] = f.w;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[i][j] = j < left ? __ldg(sx[j] + c * step) : 0.f;
+                    for (int j = 0; j < 4; ++j) v[i][j] = j < left ? __ldg(sx[j] + c * step) : 1.f;  // 1: rows that there are not
                 }
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h) w[i][h] = __ldg(sw[h] + c);
             }
             if (!mbar_wait_warp(sfree + at.stage, at.phase ^ 1u)) return false;
             float* to = slots + at.stage * 4 * f8_slot_floats(BN) + 4 * lane;
+            float least = 1.f, most = 1.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-                    *reinterpret_cast<float4*>(to + i * f8_slot_floats(BN) + h * kGroupRows) =
-                        make_float4(v[i][0] * w[i][h], v[i][1] * w[i][h], v[i][2] * w[i][h], v[i][3] * w[i][h]);
+                for (int h = 0; h < kHalves; ++h) {
+                    const float4 p = make_float4(v[i][0] * w[i][h], v[i][1] * w[i][h], v[i][2] * w[i][h], v[i][3] * w[i][h]);
+                    *reinterpret_cast<float4*>(to + i * f8_slot_floats(BN) + h * kGroupRows) = p;
+                    least = fminf(fminf(least, fminf(fabsf(p.x), fabsf(p.y))), fminf(fabsf(p.z), fabsf(p.w)));
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(p.x), fabsf(p.y))), fmaxf(fabsf(p.z), fabsf(p.w)));
+                }
+            const bool odd = __any_sync(kFullMask, !is_normal(least) || !is_normal(most));
+            if (lane == 0) apart[at.stage] = odd;
             __syncwarp();
             if (lane == 0) mbar_arrive(sfull + at.stage);
             at.next();
@@ -243,7 +259,7 @@ __device__ __forceinline__ void f8_bring_out(const F8Args& a, const F8Tile& x, f
 
 template <int BN, int CTAS, bool SPLIT>
 __device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, uint64_t* done, uint64_t* taken, const float* slots,
-                                               uint64_t* sfull, uint64_t* sfree, unsigned char* ring_ptr, unsigned char* staging,
+                                               const int* s_apart, uint64_t* sfull, uint64_t* sfree, unsigned char* ring_ptr, unsigned char* staging,
                                                int t0, int stride, int tiles, int rank, int ranks) {
     constexpr bool PAIR = CTAS == 2;
     constexpr int A = f8_accs(BN), HALF = BN / 2;  // HALF: columns of an output warp
@@ -273,11 +289,18 @@ __device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, u
 #pragma unroll
             for (int h = 0; h < 2 && h < kReads; ++h) tmem_ld32(from + at.stage * BN + 32 * h, v[h]);
         }
-#pragma unroll 1
-        for (int c = x.c0; c < x.c1; ++c) {
+        // One stage; APART: some row's two scales may have to be multiplied one after the other.
+        auto stage = [&](auto odd, int c) {
+            constexpr bool APART = decltype(odd)::value;
             const int in_group = (c - x.c0) & 3;
-            if (in_group == 0 && !mbar_wait_warp(sfull + sat.stage, sat.phase)) return false;
-            const float scale = my_scale[(sat.stage * 4 + in_group) * f8_slot_floats(BN)];
+            float scale = my_scale[(sat.stage * 4 + in_group) * f8_slot_floats(BN)], before = 1.f;
+            if (APART && !is_normal(scale)) {
+                const int tile = min(x.col0 / kF8K + (BN == 256 ? half : 0), a.R - 1);
+                const float sx = my_row < 0 ? 1.f : __ldg(a.x_scale + (a.scale_ld ? x.place + r + c * a.scale_ld : (int64_t)my_row * a.C + c));
+                const float sw = my_row < 0 ? 1.f : __ldg(a.w_scale + ((int64_t)x.bucket * a.R + tile) * a.C + c);
+                before = fabsf(sx) < fabsf(sw) ? sw : sx;
+                scale = fabsf(sx) < fabsf(sw) ? sx : sw;
+            }
             const bool more = c + 1 < x.c1;
             const int now = at.stage;
             at.next();
@@ -298,6 +321,10 @@ __device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, u
                         if (in_group == 3 || !more) mbar_arrive(sfree + sat.stage);
                     }
                 }
+                if (APART) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[h & 1][j] = __float_as_uint(__uint_as_float(v[h & 1][j]) * before);
+                }
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) fma2(acc[32 * h + j], acc[32 * h + j + 1], v[h & 1][j], v[h & 1][j + 1], scale);
                 if (h + 2 < kReads) {
@@ -311,6 +338,21 @@ __device__ __forceinline__ bool f8_output_role(const F8Args& a, uint32_t tmem, u
                 }
             }
             if (in_group == 3 || !more) sat.next();
+            return true;
+        };
+        int c = x.c0;
+#pragma unroll 1
+        for (; c < x.c1; ++c) {
+            if (((c - x.c0) & 3) == 0) {
+                if (!mbar_wait_warp(sfull + sat.stage, sat.phase)) return false;
+                if (s_apart[sat.stage]) break;
+            }
+            if (!stage(std::false_type(), c)) return false;
+        }
+#pragma unroll 1
+        for (; c < x.c1; ++c) {  // from the first group with such scales on
+            if (((c - x.c0) & 3) == 0 && !mbar_wait_warp(sfull + sat.stage, sat.phase)) return false;
+            if (!stage(std::true_type(), c)) return false;
         }
         if (SPLIT) {
             // the last accumulator is complete, so nothing reads the ring any more: it takes the partial tile
@@ -375,6 +417,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
     uint64_t* sfree = sfull + kF8Groups;                                        // [kF8Groups] and has been read
     uint64_t* drained = sfree + kF8Groups;                                      // [1]
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drained + 1);
+    int* s_apart = reinterpret_cast<int*>(s_tmem + 1);                          // [kF8Groups] a product of two scales of the group is not normal
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int rank = 0, ranks = 1;
@@ -423,7 +466,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
             if (!(PAIR && rank != 0))
                 ok = f8_issue_role<BN, CTAS, SPLIT>(a, tmem, ring, full, empty, done, taken, drained, t0, stride, tiles, rank, ranks);
         } else if (warp == 2) {
-            ok = f8_scale_role<BN, CTAS, SPLIT>(a, slots, sfull, sfree, t0, stride, tiles, rank, ranks);
+            ok = f8_scale_role<BN, CTAS, SPLIT>(a, slots, s_apart, sfull, sfree, t0, stride, tiles, rank, ranks);
         }
         __syncwarp();
         if (!ok && lane == 0) note_timeout(a.status);
@@ -433,7 +476,7 @@ __global__ void __launch_bounds__(kF8Threads, 1)
         }
     } else {
         if (BN == 256) more_registers<kF8ManyRegs>();
-        const bool ok = f8_output_role<BN, CTAS, SPLIT>(a, tmem, done, taken, slots, sfull, sfree, ring_ptr, staging, t0, stride, tiles, rank, ranks);
+        const bool ok = f8_output_role<BN, CTAS, SPLIT>(a, tmem, done, taken, slots, s_apart, sfull, sfree, ring_ptr, staging, t0, stride, tiles, rank, ranks);
         if (!ok && lane == 0) note_timeout(a.status);
         if (SPLIT) {
             __syncwarp();
