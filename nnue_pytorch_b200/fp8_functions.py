@@ -5,7 +5,8 @@ scale per 128 x 128 tile of each bucket's matrix).  Scales are powers of two: 2^
 largest finite number is a (MAX 448 for e4m3, 57344 for e5m2), 1 for a block of zeros; the only rounding is the one to
 8 bits.  Numbers that are not finite become NaN in e4m3 and stay what they are in e5m2, without touching the scale.
 
-`linear_fp8` multiplies them, dense or bucketed (with a `GroupPlan`), for evaluation: it has no gradient.
+`linear_fp8` multiplies them, dense or bucketed (with a `GroupPlan`), for evaluation: it has no gradient.  Blocks are constants:
+quantised weights do not lead back to the parameters they were made of, and rows that would need a gradient are refused.
 
     w8 = quantize_fp8_tiles(weight, count)               # once per export
     y = linear_fp8(x, w8, bias, plan)                    # x bf16, fp16 or fp32: quantised on the way in
@@ -17,7 +18,7 @@ import torch
 
 from . import _lib
 from ._launch import _outside_graphs, _ptr, _require_cuda, _span, _stream
-from .grouped_linear_functions import GATHERED_ROWS, TYPES, GroupPlan, _on, _pitched, _rows
+from .grouped_linear_functions import GATHERED_ROWS, TYPES, GroupPlan, _has_tangent, _on, _pitched, _rows
 
 FORMATS = (torch.float8_e4m3fn, torch.float8_e5m2)
 BLOCK = 128
@@ -61,6 +62,11 @@ def _check_source(t: torch.Tensor, format: torch.dtype) -> None:
     assert format in FORMATS, "float8_e4m3fn or float8_e5m2"
 
 
+def _check_no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
+    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    assert not wanted and not _has_tangent(*tensors), f"{what} has no gradient: call it under torch.no_grad()"
+
+
 def _empty_q(rows: int, K: int, format: torch.dtype, dev) -> tuple[torch.Tensor, int]:
     pitch = (K + 15) // 16 * 16
     q = torch.empty(rows, pitch, dtype=format, device=dev)
@@ -69,7 +75,8 @@ def _empty_q(rows: int, K: int, format: torch.dtype, dev) -> tuple[torch.Tensor,
 
 @_outside_graphs
 def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
-    """x [T, K] (fp32, bf16 or fp16) in 8 bits, one scale per 128 consecutive numbers of a row."""
+    """x [T, K] (fp32, bf16 or fp16) in 8 bits, one scale per 128 consecutive numbers of a row.  Has no gradient."""
+    _check_no_gradient("quantize_fp8_rows", x)
     dev = _require_cuda(x)
     _check_source(x, format)
     x, ldx = _rows(x.detach())
@@ -86,7 +93,8 @@ def quantize_fp8_rows(x: torch.Tensor, format: torch.dtype = torch.float8_e4m3fn
 @_outside_graphs
 def quantize_fp8_tiles(weight: torch.Tensor, count: int = 1, format: torch.dtype = torch.float8_e4m3fn) -> Fp8Blocks:
     """weight [count * N, K] (fp32, bf16 or fp16; `count` matrices below one another) in 8 bits, one scale per tile of
-    128 x 128 of each matrix."""
+    128 x 128 of each matrix.  The blocks are constants, also those of a parameter."""
+    assert not _has_tangent(weight), "quantize_fp8_tiles has no gradient: no tangent passes it"
     dev = _require_cuda(weight)
     _check_source(weight, format)
     count = int(count)
@@ -115,9 +123,7 @@ def linear_fp8(x: torch.Tensor | Fp8Blocks, weight: Fp8Blocks, bias: torch.Tenso
     plan    the rows' `GroupPlan`; None for a single matrix (count 1)
     out_dtype  float32, bfloat16 or float16; x's type by default (bfloat16 for `Fp8Blocks`)"""
     assert isinstance(weight, Fp8Blocks) and weight.scale.dim() == 3, "the weight is an Fp8Blocks of tiles"
-    assert not torch.is_grad_enabled() or not (
-        (isinstance(x, torch.Tensor) and x.requires_grad) or (bias is not None and bias.requires_grad)), \
-        "linear_fp8 has no gradient: call it under torch.no_grad()"
+    _check_no_gradient("linear_fp8", x if isinstance(x, torch.Tensor) else x.scale, weight.scale, bias)
     format = weight.q.dtype
     E = weight.scale.shape[0]
     given = not isinstance(x, torch.Tensor)

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import torch
 from torch import autograd
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -28,6 +29,11 @@ HALF = (torch.bfloat16, torch.float16)
 def _on(dev: torch.device):
     """Context in which `dev` is the current device (nothing to do when it already is)."""
     return _NO_SPAN if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """True inside a forward-mode level where one of the tensors carries a tangent (such a tensor need not require a gradient)."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _pad4(n: int) -> int:
@@ -219,8 +225,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     out_dtype  x's type (default) or float32
 
     Gradients: those of the formula, with dy rounded to x's type where it is fp32; each in its tensor's own type.  They have
-    no gradients of their own.  Everything runs on the current stream and can be captured into a CUDA graph; as for any
+    no gradients of their own, and there is no forward mode: tensors with tangents are refused.  Everything runs on the current stream and can be captured into a CUDA graph; as for any
     operator, no eager autograd graph of the same leaves may be alive when a backward pass is captured."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))) \
+            or _has_tangent(x, weight, bias):  # the function has no forward mode and says so
         return GroupedLinearFunction.apply(x, weight, bias, plan, out_dtype)
     return _forward(x, weight, bias, plan, out_dtype, False)[0]

@@ -23,14 +23,15 @@ class _Recorder:
 
 @pytest.fixture
 def recorder(monkeypatch):
-    """`grouped_linear` on CPU tensors: its checks and its calls, no kernel."""
-    from nnue_pytorch_b200 import grouped_linear_functions as gl
+    """The operators on CPU tensors: their checks and their calls, no kernel."""
+    from nnue_pytorch_b200 import fp8_functions, grouped_linear_functions
 
     lib = _Recorder()
-    monkeypatch.setattr(gl._lib, "load", lambda: lib)
-    monkeypatch.setattr(gl, "_require_cuda", lambda *tensors: tensors[0].device)
-    monkeypatch.setattr(gl, "_on", lambda dev: contextlib.nullcontext())
-    monkeypatch.setattr(gl, "_stream", lambda dev: 0)
+    monkeypatch.setattr(grouped_linear_functions._lib, "load", lambda: lib)
+    for module in (grouped_linear_functions, fp8_functions):
+        monkeypatch.setattr(module, "_require_cuda", lambda *tensors: tensors[0].device)
+        monkeypatch.setattr(module, "_on", lambda dev: contextlib.nullcontext())
+        monkeypatch.setattr(module, "_stream", lambda dev: 0)
     return lib
 
 
@@ -81,3 +82,42 @@ def test_waits_for_tensor_memory_name_their_registers():
             named = wait.group(1).count('"+r"')
             assert named == 32, f"{name}: the wait for a read of 32 registers names {named}"
         assert "tmem_wait_ld()" not in source, name
+
+
+def test_forward_mode_is_refused(recorder):
+    """A dual tensor does not require a gradient; its tangent may not get lost, with gradients on or off."""
+    from torch.autograd import forward_ad
+
+    from nnue_pytorch_b200 import Fp8Blocks, grouped_linear, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
+
+    x, w, bias = torch.zeros(4, 64), torch.zeros(2 * 8, 64), torch.zeros(2 * 8)
+    w8 = Fp8Blocks(torch.zeros(8, 64).to(torch.float8_e4m3fn), torch.ones(1, 1, 1))
+    for mode in (contextlib.nullcontext, torch.no_grad):
+        with mode(), forward_ad.dual_level():
+            for i in range(3):
+                args = [t.bfloat16() for t in (x, w, bias)]
+                args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                assert not args[i].requires_grad
+                with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                    grouped_linear(*args, _plan(4, 2))
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            for call in (lambda: quantize_fp8_rows(dual), lambda: quantize_fp8_tiles(dual), lambda: linear_fp8(dual, w8),
+                         lambda: linear_fp8(x, w8, forward_ad.make_dual(bias[:8], bias[:8]))):
+                with pytest.raises(AssertionError, match="no gradient"):
+                    call()
+            assert grouped_linear(x.bfloat16(), w.bfloat16(), None, _plan(4, 2)).shape == (4, 8)  # no tangent: as ever
+            assert linear_fp8(x, w8).shape == (4, 8)
+
+
+def test_rows_that_need_a_gradient_are_not_quantised(recorder):
+    from nnue_pytorch_b200 import Fp8Blocks, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
+
+    x = torch.zeros(4, 64, requires_grad=True)
+    with pytest.raises(AssertionError, match="no gradient"):
+        quantize_fp8_rows(x)
+    with torch.no_grad():
+        assert quantize_fp8_rows(x).q.shape == (4, 64)
+    blocks = quantize_fp8_tiles(torch.nn.Parameter(torch.zeros(4, 64)))  # weights are exported as constants
+    assert not blocks.q.requires_grad and not blocks.scale.requires_grad
+    with pytest.raises(AssertionError, match="no gradient"):  # scales of one's own
+        linear_fp8(torch.zeros(4, 64), Fp8Blocks(blocks.q, torch.ones(1, 1, 1, requires_grad=True)))
