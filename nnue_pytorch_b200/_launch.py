@@ -88,9 +88,12 @@ def get_backward_mode() -> str:
     return _BWD_MODE
 
 
-def _stream(device: torch.device) -> int:
-    # the same number as torch.cuda.current_stream(device).cuda_stream, without the Stream object (3 us)
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _stream(device: torch.device | str | int | None) -> int:
+    # the same number as torch.cuda.current_stream(device).cuda_stream; without the Stream object (3 us) where the device is a
+    # tensor's and so has an index
+    if isinstance(device, torch.device) and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _outside_graphs(fn):

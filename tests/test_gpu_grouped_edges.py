@@ -105,3 +105,14 @@ def test_very_long_sums_in_16_bits(dev, direction):
     else:
         dw, = torch.autograd.grad(y, w, dy.detach() / small)
         _near(dw, (dy.detach() / small).double().T @ x.detach().double(), long, "dw")
+
+
+def test_status_of_a_device_without_an_index(dev):
+    from nnue_pytorch_b200 import _launch
+
+    for device in (None, torch.device("cuda"), "cuda", "cuda:0", 0):
+        _launch.device_status(device)
+        assert _launch._stream(device) == torch.cuda.current_stream(device).cuda_stream
+    side = torch.cuda.Stream(dev)
+    with torch.cuda.stream(side):
+        assert _launch._stream(torch.device("cuda")) == _launch._stream(dev) == side.cuda_stream

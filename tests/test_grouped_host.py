@@ -121,3 +121,14 @@ def test_rows_that_need_a_gradient_are_not_quantised(recorder):
     assert not blocks.q.requires_grad and not blocks.scale.requires_grad
     with pytest.raises(AssertionError, match="no gradient"):  # scales of one's own
         linear_fp8(torch.zeros(4, 64), Fp8Blocks(blocks.q, torch.ones(1, 1, 1, requires_grad=True)))
+
+
+def test_stream_of_a_device_without_an_index(monkeypatch):
+    """`device_status` and others pass on the device they are given: without an index, a string, a number or none."""
+    from nnue_pytorch_b200 import _launch
+
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: types.SimpleNamespace(cuda_stream=("stream of", device)))
+    assert _launch._stream(torch.device("cuda", 3)) == 103
+    for device in (torch.device("cuda"), "cuda", "cuda:0", 0, None):
+        assert _launch._stream(device) == ("stream of", device)
