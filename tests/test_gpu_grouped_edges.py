@@ -116,3 +116,50 @@ def test_status_of_a_device_without_an_index(dev):
     side = torch.cuda.Stream(dev)
     with torch.cuda.stream(side):
         assert _launch._stream(torch.device("cuda")) == _launch._stream(dev) == side.cuda_stream
+
+
+# Tiles of every width, of one CTA and of pairs, split and whole, in each direction: (rows, buckets, inputs, outputs), and the
+# columns of the tiles that 148 SMs get in forward, dx and dw.
+FORMS = [
+    (24000, 8, 512, 1000),  # pairs, pairs, 128
+    (3000, 8, 2560, 264),  # 32, pairs, pairs
+    (4000, 40, 1000, 1000),  # 256, 256, pairs
+    (3000, 40, 1000, 100),  # 32, 256, 256
+    (2000, 20, 1000, 1000),  # 128, 128, pairs
+    (3000, 20, 1000, 100),  # 32, pairs, 128
+    (1000, 10, 1000, 1000),  # 64, 64, pairs
+    (800, 8, 1000, 600),  # 32, 64, pairs
+    (3000, 8, 1000, 100),  # 32, 128, 64
+    (12000, 3, 4096, 72),  # 64, pairs, 64
+    (3000, 2, 300, 40),  # 32 split in 2, 64, 64 split in 8
+    (100, 2, 300, 600),  # 32 split in 2, 64 split in 4, 64
+]
+
+
+@pytest.mark.parametrize("weights", ["own", "fp32"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,count,K,N", FORMS)
+def test_whole_numbers_in_every_form(dev, T, count, K, N, dtype, weights):
+    """Whole numbers of at most 2 in size: no sum reaches 2^24, so every sum is exact in fp32, in any order and where
+    additions cut off, and each result is the 64-bit one rounded once."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator(device=dev).manual_seed(T + K + N)
+    whole = lambda *shape: torch.randint(-2, 3, shape, generator=g, device=dev).float()  # noqa: E731
+    x, w, bias, dy = whole(T, K), whole(count * N, K), whole(count * N), whole(T, N)
+    b = torch.randint(-1, count, (T,), generator=g, device=dev)
+    w_dtype = torch.float32 if weights == "fp32" else dtype
+    xd, wd, bd = x.to(dtype).requires_grad_(True), w.to(w_dtype).requires_grad_(True), bias.to(w_dtype).requires_grad_(True)
+    y = grouped_linear(xd, wd, bd, GroupPlan(b, count))
+    dx, dw, db = torch.autograd.grad(y, (xd, wd, bd), dy.to(dtype))
+    y32 = grouped_linear(xd.detach(), wd.detach(), bd.detach(), GroupPlan(b, count), out_dtype=torch.float32)
+    x, w, dy = x.double(), w.double().view(count, N, K), dy.double()
+    for e in range(count):
+        r = torch.nonzero(b == e).view(-1)
+        ref = x[r] @ w[e].T + bias.view(count, N)[e].double()
+        assert torch.equal(y[r], ref.to(dtype)) and torch.equal(y32[r].double(), ref), f"y of bucket {e}"
+        assert torch.equal(dx[r], (dy[r] @ w[e]).to(dtype)), f"dx of bucket {e}"
+        assert torch.equal(dw.view(count, N, K)[e], (dy[r].T @ x[r]).to(w_dtype)), f"dw of bucket {e}"
+        assert torch.equal(db.view(count, N)[e], dy[r].sum(0).to(w_dtype)), f"dbias of bucket {e}"
+    none = b < 0
+    assert not y[none].any() and not y32[none].any() and not dx[none].any()
