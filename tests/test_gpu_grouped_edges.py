@@ -163,3 +163,104 @@ def test_whole_numbers_in_every_form(dev, T, count, K, N, dtype, weights):
         assert torch.equal(db.view(count, N)[e], dy[r].sum(0).to(w_dtype)), f"dbias of bucket {e}"
     none = b < 0
     assert not y[none].any() and not y32[none].any() and not dx[none].any()
+
+
+def test_plan_and_8_bit_layer_inside_a_compiled_model(dev):
+    """A plan depends on the batch, so a compiled model makes its own; the 8-bit layer runs in one too."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear, linear_fp8, quantize_fp8_tiles
+
+    g = torch.Generator().manual_seed(61)
+    count, K, N = 4, 48, 24
+    w = torch.randn(count * N, K, generator=g).to(dev).requires_grad_(True)
+    w8 = quantize_fp8_tiles(w, count)
+
+    def train(x, b, w):
+        return grouped_linear(x * 2, w, None, GroupPlan(b, count)).clamp(0, 1) * 3
+
+    def evaluate(x, b):
+        return linear_fp8(x * 2, w8, None, GroupPlan(b, count)).clamp(0, 1) * 3
+
+    compiled = torch.compile(train, backend="eager"), torch.compile(evaluate, backend="eager")
+    for T in (200, 200, 37):  # the second batch runs what the first compiled, the third has another length
+        b = torch.randint(-1, count, (T,), generator=g).to(dev)
+        x = torch.randn(T, K, generator=g).bfloat16().to(dev).requires_grad_(True)
+        want, got = train(x, b, w), compiled[0](x, b, w)
+        assert torch.equal(want, got)
+        for p, q in zip(torch.autograd.grad(want.sum(), (x, w)), torch.autograd.grad(got.sum(), (x, w))):
+            assert torch.equal(p, q)
+        with torch.no_grad():
+            assert torch.equal(evaluate(x, b), compiled[1](x, b))
+
+
+def test_two_captured_graphs_replayed_in_any_order(dev):
+    """Two graphs of one process, each with a plan, both directions and the 8-bit layer, replayed in turn and side by side on
+    two streams: they share no buffer."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear, linear_fp8, quantize_fp8_tiles
+
+    def inputs(T, count, K, N, seed):
+        g = torch.Generator().manual_seed(seed)
+        return (torch.randint(-1, count, (T,), generator=g).to(dev), torch.randn(T, K, generator=g).bfloat16().to(dev),
+                torch.randn(count * N, K, generator=g).to(dev), torch.randn(T, N, generator=g).bfloat16().to(dev), count)
+
+    def step(b, x, w, dy, count):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        plan = GroupPlan(b, count)
+        y = grouped_linear(x, w, None, plan)
+        out = (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+        with torch.no_grad():
+            return (*out, linear_fp8(x, quantize_fp8_tiles(w, count), None, plan))
+
+    data = [inputs(3000, 3, 256, 300, 71), inputs(900, 8, 320, 96, 72)]
+    want = [step(*d) for d in data]
+    graphs, outs = [], []
+    for d in data:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*d))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(dev) for _ in data]
+    for order in ((0, 1), (1, 0), (0, 0), (1, 1)):
+        for t in (t for o in outs for t in o):
+            t.fill_(7)
+        torch.cuda.synchronize()
+        for i in order:
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in set(order):
+            assert all(torch.equal(p, q) for p, q in zip(want[i], outs[i]))
+    del graphs
+
+
+@pytest.mark.parametrize("T", [30, 3000])
+def test_broadcast_weights_and_repeated_leaves(dev, T):
+    """One matrix expanded over all buckets, its gradient the sum over them; the same layer twice in a graph; checkpointed."""
+    from torch.utils.checkpoint import checkpoint
+
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear
+
+    g = torch.Generator(device=dev).manual_seed(81)
+    count, K = 5, 72
+    whole = lambda *shape: torch.randint(-1, 2, shape, generator=g, device=dev).float()  # noqa: E731
+    b = torch.randint(-1, count, (T,), generator=g, device=dev)
+    plan = GroupPlan(b, count)
+    x = (whole(T, K) * (torch.rand(T, K, generator=g, device=dev) < 0.1)).bfloat16().requires_grad_(True)
+    one = whole(K, K).requires_grad_(True)
+    dy = whole(T, K).bfloat16()
+
+    def twice(x, one):
+        w = one.expand(count, K, K)
+        return grouped_linear(grouped_linear(x, w, None, plan), w, None, plan, out_dtype=torch.float32)
+
+    live = (b >= 0).double()[:, None]
+    h = (x.detach().double() @ one.detach().double().T) * live
+    want = (h @ one.detach().double().T) * live
+    dh = (dy.double() * live) @ one.detach().double()
+    assert h.abs().max() < 256 and dh.abs().max() < 256  # exact in bf16 on the way
+    dx, dw = dh @ one.detach().double() * live, (dy.double() * live).T @ h + dh.T @ (x.detach().double() * live)
+    for run in (twice, lambda x, one: checkpoint(twice, x, one, use_reentrant=False)):
+        y = run(x, one)
+        got = torch.autograd.grad(y, (x, one), dy.float())
+        assert torch.equal(y.double(), want)
+        assert torch.equal(got[0], dx.bfloat16()) and torch.equal(got[1].double(), dw)
