@@ -817,8 +817,9 @@ int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
  *                 sum_{k in block c} x[p, k] w[b, n, k]  + bias[b, n]
  * x [T, K] and w [E, N, K] of one 8-bit format, pitches that are multiples of 16,
  * scales as the quantisers lay them out (x_scale with the same scale_ld; by place
- * with rows laid out by bucket or one matrix; any fp32 values, not only powers of two), bias [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are
- * fp32.  plan NULL: E = 1 and every row belongs to the one matrix.  With a plan, x
+ * with rows laid out by bucket or one matrix; any fp32 values, not only powers of two:
+ * where x_scale w_scale is not a normal number the larger one is applied first), bias
+ * [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are fp32.  plan NULL: E = 1 and every row belongs to the one matrix.  With a plan, x
  * is laid out by bucket (`laid`; ldx is not looked at) or in the batch's order,
  * which suits a few rows per bucket. */
 int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid,

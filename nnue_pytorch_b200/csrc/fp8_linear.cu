@@ -8,9 +8,9 @@
 // and so is the weights' on its columns); another warp fetches the scales, which may be any fp32 numbers.
 // Bound by the way of an accumulator, not by the tensor core: a stage of a pair of SMs on 256 x 256 multiplies in 390 cycles,
 // but its first result is there after 900, is read and scaled in 700 to 900 and given back in 240, and tensor memory holds
-// two: about 1000 cycles per stage (16384 x 4096 x 2048 over 8 buckets: 175 us, 1.57 PFLOP/s; 135 us of it are stages at
-// work, 20 to 40 the bringing out of eight tiles per pair; 180 with the test of the scales below).  Four accumulators of 128 columns halve the way but double the stages
-// (223 us), and two products of 128 columns per stage came to 219.
+// two: about 1000 cycles per stage (16384 x 4096 x 2048 over 8 buckets: 180 us, 1.53 PFLOP/s; 135 us of it are stages at
+// work, 20 to 40 the bringing out of eight tiles per pair).  Four accumulators of 128 columns halve the way but double the
+// stages (223 us, when 256 columns took 178), and two products of 128 columns per stage came to 219.
 // Copies, pairs of SMs, split sums and bounded waits as in the 16-bit kernel (grouped_linear.cu).  Rows come laid out by
 // bucket (the quantiser leaves them so), in their own order where there is one matrix, or are gathered by TMA, four per
 // copy, where a bucket has few.
@@ -524,9 +524,12 @@ int f8_launch(const CUtensorMap& mx, const CUtensorMap& mw, const F8Args& a, int
     return NNUE_OK;
 }
 
-// Pairs on 256 columns or CTAs on up to 128.  A round of the latter takes about 5/8 of a pair's round for half the work: at
-// 4099 x 2000 x 1500 two rounds of pairs, 1.4 full, came to 55 us and three of single CTAs, 2.7 full, to 50; at 16384 x 4096
-// x 2048 over 8 buckets eight rounds of pairs to 175 us, against 223 for pairs on 128 columns.
+// Pairs on 256 columns or CTAs on up to 128.  A round of the latter takes about 5/8 of a pair's round for half the work.
+// Pairs and single CTAs, us, the kept one first:
+//   pairs   2048 x 4096 x 2048 28, 35      4096 x 4096 x 4096 89, 102      16384 x 4096 x 2048 over 8 even buckets 157, 203
+//           8192 x 2048 x 512 over 8 21, 23      16384 x 512 x 512 over 8 18.5 to 19.5, 17.8 (the rule's one miss of these)
+//   single  4099 x 2000 x 1500 49, 54      20000 x 1000 x 520 over 3 34, 38      6000 x 1024 x 1000 over 2 21, 24
+// Pairs on 128 columns took 223 for 180 at 16384 x 4096 x 2048 over 8 uneven buckets.
 static TileShape f8_shape(int64_t runs, int64_t T, int64_t N, int64_t chunks, bool pairs) {
     const int64_t rows = (T + runs - 1) / runs, sms = sm_count();
     auto rounds = [&](int64_t high, int64_t wide, int64_t at_once) {

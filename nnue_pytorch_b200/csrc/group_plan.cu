@@ -3,7 +3,8 @@
 //
 // Mathematics: place(p) = #{q : b(q) < b(p)} + #{q < p : b(q) = b(p)}.  A warp takes 32 consecutive rows at a time, so
 // the second term is a histogram of the rows before its slice plus the lanes below it that hold the same bucket
-// (one match instruction).  Work: ids read twice, order written once; bound by latency up to about a million rows.
+// (one match instruction).  Work: ids read twice (three times in the form for long batches), order written once; bound by
+// latency up to about a million rows.
 //
 // Three forms, all with a counter per warp and bucket in shared memory, blocks of 1024 threads:
 //   up to   2048 rows  one block                                                          (2048 rows, 8 buckets: 10 us)

@@ -37,7 +37,9 @@ __host__ __device__ inline int64_t group_max_tiles(int64_t T, int32_t E) {
     return by_rows < T ? by_rows : T;  // every tile holds a row
 }
 
-// rows of a buffer that holds a batch laid out by bucket, and room behind it for a whole tile of any bucket
+// Rows of a buffer that holds a batch laid out by bucket: it ends with the last bucket's multiple of kGroupAlign rows, at the
+// most.  A tile's box of 128 rows may reach behind it: the tensor map has this number of rows, and what lies behind reads as
+// zeros.  Plain loads have to stay below the tile's count, rounded up to kGroupAlign.
 __host__ __device__ inline int64_t group_laid_rows(int64_t T, int32_t E) {
     return T + (int64_t)(kGroupAlign - 1) * (E < T ? E : T);
 }

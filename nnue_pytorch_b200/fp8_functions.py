@@ -63,8 +63,11 @@ def _check_source(t: torch.Tensor, format: torch.dtype) -> None:
 
 
 def _check_no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
-    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-    assert not wanted and not _has_tangent(*tensors), f"{what} has no gradient: call it under torch.no_grad()"
+    wanted = _has_tangent(*tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            wanted |= t is not None and t.requires_grad
+    assert not wanted, f"{what} has no gradient: call it under torch.no_grad()"
 
 
 def _empty_q(rows: int, K: int, format: torch.dtype, dev) -> tuple[torch.Tensor, int]:

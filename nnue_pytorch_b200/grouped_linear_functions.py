@@ -106,11 +106,7 @@ def _pitched(t: torch.Tensor, dtype: torch.dtype, lib, dev, whole: bool = False)
     t, ld = _rows(t)
     pitch = (cols + unit - 1) // unit * unit
     out = torch.empty(rows, pitch, dtype=dtype, device=dev)
-    if t.dtype.itemsize != 1:
-        st = lib.nnue_pack_rows(_ptr(t), TYPES[t.dtype], ld, _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
-    else:
-        assert t.dtype == dtype
-        st = lib.nnue_pack_rows(_ptr(t), TYPES[dtype], ld, _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
+    st = lib.nnue_pack_rows(_ptr(t), TYPES[t.dtype], ld, _ptr(out), TYPES[dtype], pitch, rows, cols, _stream(dev))
     _lib.check(st, "nnue_pack_rows")
     return out, pitch
 
@@ -127,13 +123,17 @@ def _laid_out(t: torch.Tensor, dtype: torch.dtype, plan_buffer, E: int, lib, dev
     return out, part
 
 
-# Up to this many rows per bucket the products gather them as they lie; beyond it they are laid out by bucket first.
+# Up to this many rows per bucket the products gather them as they lie; beyond it they are laid out by bucket first.  Kernels
+# together, us, gathered against laid out (8 bits in brackets):
+#   8 buckets of 1024 -> 1024, bf16     16 rows 21, 26 (18, 20)    32 rows 25, 26 (19, 20)    64 rows 33, 29 (22, 20)
+#   64 of 2048 -> 1024                  16 rows 65, 73 (51, 53)    32 rows 66, 75 (58, 54)    64 rows 72, 78 (77, 56)
+#   8 of 4096 -> 2048                    8 rows 53, 57 (40, 40)    16 rows 61, 57 (44, 40)    32 rows 78, 58 (52, 40)
 GATHERED_ROWS = 16
 
 
 def _forward(x, weight, bias, plan, out_dtype, keep_rows):
-    """y, x as the product read it and the weights as it read them.  `keep_rows`: x is laid out by bucket whatever its
-    length, as the weight gradient reads it."""
+    """y, x as the product read it, the weights as it read them and their pitch.  `keep_rows`: x is laid out by bucket whatever
+    its length, as the weight gradient reads it."""
     dev = _require_cuda(x, weight) if bias is None else _require_cuda(x, weight, bias)
     dtype = x.dtype
     assert dtype in HALF, "rows are bf16 or fp16"
@@ -165,15 +165,15 @@ def _forward(x, weight, bias, plan, out_dtype, keep_rows):
             _ptr(xr), ldx, laid, _ptr(wr), ldw, _ptr(bias), 0 if bias is None else TYPES[bias.dtype], _ptr(plan.buffer), _ptr(y),
             TYPES[out_dtype], T, K, N, E, TYPES[dtype], s)
     _lib.check(st, "nnue_grouped_linear_fwd")
-    return y, xr, wr
+    return y, xr, wr, ldw
 
 
 class GroupedLinearFunction(autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, plan, out_dtype=None):
-        y, xr, wr = _forward(x, weight, bias, plan, out_dtype, ctx.needs_input_grad[1])
+        y, xr, wr, ldw = _forward(x, weight, bias, plan, out_dtype, ctx.needs_input_grad[1])
         ctx.save_for_backward(xr if ctx.needs_input_grad[1] else None, wr if ctx.needs_input_grad[0] else None, plan.buffer)
-        ctx.dims = (*x.shape, y.shape[1], plan.count)
+        ctx.dims, ctx.w_read = (*x.shape, y.shape[1], plan.count), (wr.stride(), ldw)
         ctx.dtype, ctx.w_like, ctx.b_like = x.dtype, (weight.dtype, weight.shape), None if bias is None else (bias.dtype, bias.shape)
         return y
 
@@ -197,7 +197,9 @@ class GroupedLinearFunction(autograd.Function):
                 dyr, lddy = _pitched(dy, dtype, lib, dev)
                 laid = 0
             if need_x:
-                w, ldw = _pitched(w, dtype, lib, dev)
+                strides, ldw = ctx.w_read
+                if w.stride() != strides:
+                    w, ldw = _pitched(w, dtype, lib, dev)
                 dx = torch.empty(T, K, dtype=dtype, device=dev)
                 _lib.check(lib.nnue_grouped_linear_bwd_input(_ptr(dyr), lddy, laid, _ptr(w), ldw, _ptr(plan), _ptr(dx), T, K, N, E,
                                                              TYPES[dtype], s), "nnue_grouped_linear_bwd_input")
