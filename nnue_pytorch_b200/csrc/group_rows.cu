@@ -3,6 +3,8 @@
 // every tile of 128 rows can be taken (the bias gradient of a linear layer: dbias[b] = sum of its rows of dy).
 //
 // Bound by HBM: every row is read and written once; a warp moves rows of up to 512 bytes, four at a time in flight.
+// 16384 x 4096 bf16 51 us, 81 % of the measured copy rate; 16384 x 2048 with sums 28 us, 74 %; short rows less (8192 x 1024
+// with sums 13 us, 40 %), and rows off 16 bytes are read number by number.
 #include "grouped.cuh"
 
 namespace nnue {

@@ -12,7 +12,7 @@
 // end, and forward and dx never store the rows of a tile behind its count.  Without that layout forward and dx gather
 // four rows per copy.  A four-row copy takes an SM about 75 cycles whatever issues it (675 us for the forward of 16384 x
 // 4096 x 2048), and rows gathered by 16-byte asynchronous copies came to 36 GB/s per SM with four warps (254 us; 595 for
-// dw): laying the rows out first costs 42 us there, and both directions read them.
+// dw): laying the rows out first costs 51 us there, and both directions read them.
 //
 // Roles: warp 0 copies into a ring of stages, warp 1 issues the instructions, warps 4-11 take the accumulators and bring
 // finished tiles out while the next run of stages multiplies (two accumulators).  Persistent: a CTA (or pair) per SM walks
@@ -26,11 +26,12 @@
 //   loses what lies below a quarter of the sum's last bit, the result what lies below that bit, so an addition loses
 //   less than 5 x 2^-23 of the sum and a sum of n terms grows off by n / 16 times that.  An accumulator therefore adds up runs
 //   of 512 terms; the output warps hold the sums in registers (half a row of the tile per thread) and add the runs rounding
-//   to nearest.  In one level the sums of 16384 x 4096 x 2048 came out 9 times as far off as those of an fp32 product.
-//   Runs of 8 stages against one for the whole sum, us at that size over 8 buckets: forward 198 (183), dx 202 (197), dw 221
-//   (219); of 4 stages 213, 212, 221; of 16 193, 198, 218: a change of accumulator costs the issuing warp about 400
+//   to nearest.  Where bf16 results of 16384 x 4096 x 2048 differ from an fp32 product's, 94 % were the farther ones from 64
+//   bits in one level, half are in two.
+//   Runs of 8 stages against one for the whole sum, us at that size over 8 buckets: forward 198 (183), dx 202 (197), dw 219
+//   (217); of 4 stages 213, 212, 221; of 16 193, 198, 218: a change of accumulator costs the issuing warp about 400
 //   cycles.  dw in fp32 227 (353 with the total in tensor memory, which leaves room for 128 columns only).
-// Measured at that size, bf16: forward 198 us (1.39 PFLOP/s), dx 202, dw 221 after 81 for laying x and dy out; bound by the
+// Measured at that size, bf16: forward 198 us (1.39 PFLOP/s), dx 202, dw 219 after 51 for laying x out and 28 for dy; bound by the
 // issuing warp's way from stage to stage (about 800 cycles for 512 of multiplying) and the operands' way through L2 and
 // shared memory (32 KB per SM and stage).
 // All orders are fixed by the sizes: results are reproducible.  Every wait is bounded; one that runs out raises the
