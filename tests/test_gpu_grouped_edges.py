@@ -264,3 +264,66 @@ def test_broadcast_weights_and_repeated_leaves(dev, T):
         got = torch.autograd.grad(y, (x, one), dy.float())
         assert torch.equal(y.double(), want)
         assert torch.equal(got[0], dx.bfloat16()) and torch.equal(got[1].double(), dw)
+
+
+# ---- offsets beyond 32 bits and many rows
+@pytest.mark.parametrize("T,count", [(3_000_001, 1000), (20_000_000, 7)])
+def test_plan_of_many_rows(dev, T, count):
+    from nnue_pytorch_b200 import GroupPlan
+
+    g = torch.Generator(device=dev).manual_seed(91)
+    b = torch.randint(-1, count, (T,), generator=g, device=dev)
+    plan = GroupPlan(b, count)
+    key = torch.where(b < 0, count, b)
+    assert torch.equal(plan.order.long(), torch.sort(key, stable=True).indices)
+    sizes = torch.bincount(key, minlength=count + 1)
+    assert torch.equal(plan.offsets.long(), torch.cat([sizes.new_zeros(1), sizes[:count].cumsum(0)]))
+
+
+def test_weights_and_gradients_of_more_than_2_31_numbers(dev):
+    """1024 matrices of 2056 x 1024, in 16 and in 8 bits; rows of the first, a middle and the last bucket."""
+    from nnue_pytorch_b200 import GroupPlan, grouped_linear, linear_fp8, quantize_fp8_tiles
+
+    count, N, K, T = 1024, 2056, 1024, 96
+    g = torch.Generator(device=dev).manual_seed(92)
+    some = torch.tensor([0, 500, 1023], device=dev)
+    whole = lambda *shape: torch.randint(-2, 3, shape, generator=g, device=dev)  # noqa: E731
+    w = torch.zeros(count, N, K, dtype=torch.bfloat16, device=dev)
+    w[some] = whole(3, N, K).bfloat16()
+    w.requires_grad_(True)
+    b = some.repeat(T // 3)
+    x, dy = whole(T, K).bfloat16().requires_grad_(True), whole(T, N).bfloat16()
+    y = grouped_linear(x, w, None, GroupPlan(b, count))
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with torch.no_grad():
+        y8 = linear_fp8(x, quantize_fp8_tiles(w.flatten(0, 1), count), None, GroupPlan(b, count), torch.float32)
+        for e in some.tolist():
+            r = torch.nonzero(b == e).view(-1)
+            ref = x[r].double() @ w[e].double().T
+            assert torch.equal(y[r], ref.bfloat16()) and torch.equal(y8[r].double(), ref)  # quantising whole numbers is exact
+            assert torch.equal(dx[r], (dy[r].double() @ w[e].double()).bfloat16())
+            assert torch.equal(dw[e], (dy[r].double().T @ x[r].double()).bfloat16())
+        assert not dw[1:500].any() and not dw[501:1023].any()
+
+
+@pytest.mark.parametrize("dense", [False, True])
+def test_8_bit_rows_of_more_than_2_31_numbers(dev, dense):
+    from nnue_pytorch_b200 import GroupPlan, linear_fp8, quantize_fp8_rows, quantize_fp8_tiles
+
+    T, K, N = 1 << 20, 2064, 16
+    count = 1 if dense else 2
+    g = torch.Generator(device=dev).manual_seed(93)
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device=dev)
+    x[-200:] = torch.randint(-2, 3, (200, K), generator=g, device=dev).bfloat16()
+    w = torch.randint(-2, 3, (count * N, K), generator=g, device=dev).bfloat16()
+    b = (torch.arange(T, device=dev) >= T - 77).long() if not dense else torch.zeros(T, dtype=torch.int64, device=dev)
+    w8, plan = quantize_fp8_tiles(w, count), None if dense else GroupPlan(b, count)
+    want = torch.stack([x[p].double() @ w.view(count, N, K)[b[p]].double().T for p in range(T - 200, T)])
+    for rows in (x, quantize_fp8_rows(x)):
+        y = linear_fp8(rows, w8, None, plan, torch.float32)
+        assert not y[:-200].any() and torch.equal(y[-200:].double(), want)
+        del y
+    wide = torch.randint(-2, 3, (count * K, 16), generator=g, device=dev).bfloat16()  # the output is the large one
+    y = linear_fp8(x[:, -16:].contiguous(), quantize_fp8_tiles(wide, count), None, plan)
+    want = torch.stack([x[p, -16:].double() @ wide.view(count, K, 16)[b[p]].double().T for p in range(T - 200, T)])
+    assert not y[:-200].any() and torch.equal(y[-200:], want.bfloat16())
