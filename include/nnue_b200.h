@@ -770,9 +770,9 @@ int nnue_group_sums(const float* sums, const void* plan, void* out,
  * bias [E, N] of any of the three float types, may be NULL; y [T, N], dx [T, K] and
  * dw [E, N, K] contiguous, y and dw of `type` or F32, dx of `type`, dbias [E, N] of
  * any float type, may be NULL.  Sums are fp32 (runs of 512 terms by the tensor core,
- * whose additions cut off, and the runs added rounding to nearest), rounded once.  Rows without a
- * bucket get zeros in y and dx, whatever they hold; a bucket without rows gets
- * zeros in dw and dbias.  Sums run in an order that the sizes alone fix: results
+ * whose additions cut off, and the runs added rounding to nearest), rounded once.
+ * Rows without a bucket get zeros in y and dx, whatever they hold; a bucket without
+ * rows gets zeros in dw and dbias.  Sums run in an order that the sizes alone fix: results
  * are reproducible.  T = 0 is allowed.  `plan`: nnue_group_plan's, of the same T
  * and E. */
 int nnue_grouped_linear_fwd(const void* x, int64_t ldx, int32_t laid,
@@ -819,9 +819,10 @@ int nnue_fp8_quantize_tiles(const void* w, int32_t type, int64_t ldw, void* q,
  * scales as the quantisers lay them out (x_scale with the same scale_ld; by place
  * with rows laid out by bucket or one matrix; any fp32 values, not only powers of two:
  * where x_scale w_scale is not a normal number the larger one is applied first), bias
- * [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are fp32.  plan NULL: E = 1 and every row belongs to the one matrix.  With a plan, x
- * is laid out by bucket (`laid`; ldx is not looked at) or in the batch's order,
- * which suits a few rows per bucket. */
+ * [E, N] F32 or NULL, y [T, N] contiguous of any float type.  Sums are fp32.  plan
+ * NULL: E = 1 and every row belongs to the one matrix.  With a plan, x is laid out by
+ * bucket (`laid`; ldx is not looked at) or in the batch's order, which suits a few
+ * rows per bucket. */
 int nnue_fp8_linear_fwd(const void* x, int64_t ldx, int32_t laid,
                         const float* x_scale, int64_t scale_ld,
                         const void* w, int64_t ldw, const float* w_scale,

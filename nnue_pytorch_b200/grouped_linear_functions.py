@@ -227,8 +227,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     out_dtype  x's type (default) or float32
 
     Gradients: those of the formula, with dy rounded to x's type where it is fp32; each in its tensor's own type.  They have
-    no gradients of their own, and there is no forward mode: tensors with tangents are refused.  Everything runs on the current stream and can be captured into a CUDA graph; as for any
-    operator, no eager autograd graph of the same leaves may be alive when a backward pass is captured."""
+    no gradients of their own, and there is no forward mode: tensors with tangents are refused.  Everything runs on the
+    current stream and can be captured into a CUDA graph; as for any operator, no eager autograd graph of the same leaves
+    may be alive when a backward pass is captured."""
     if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))) \
             or _has_tangent(x, weight, bias):  # the function has no forward mode and says so
         return GroupedLinearFunction.apply(x, weight, bias, plan, out_dtype)
